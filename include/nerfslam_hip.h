@@ -35,6 +35,7 @@ extern "C" {
 
 #define NS_F16 1
 #define NS_F32 2
+#define NS_BF16 3 /* row operators only (ns_embedding_*, ns_layer_norm_*)                                    */
 
 #define NS_ACT_NONE 0
 #define NS_ACT_RELU 1
@@ -738,6 +739,37 @@ int ns_ngp_grid_update(const void* net_out, const int* cells, int n, float min_s
 int ns_ngp_grid_update_sampled(const void* net_out, const int* cells, int n, float min_step, float decay, float max_threshold,
                                float* density_grid, float* tmp_grid, long n_cells_total, double* partial_ws, unsigned char* bits,
                                void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rows of features: a table looked up by id, and layer norm (host side: nerfslam/rows.py).  dtype: NS_F16, NS_BF16 or NS_F32; sums
+ * in f32, one rounding per output.  A row is `cols` consecutive elements; `*_stride` is the distance of two rows in elements (0: the
+ * same row throughout), outputs without one are dense.  Element alignment is enough.  [no reference counterpart]
+ * ---------------------------------------------------------------------------------------- */
+
+/* out[t] = scale * table[ids[t]]; an id outside [0, rows) (a padded place) gives a row of zeros.
+ *   table [rows, cols] dtype, ids [n] int32 (int64 if ids_are_64), out [n, cols] dtype; n <= 2^27, rows <= 2^29, cols <= 65536. */
+int ns_embedding_forward(const void* table, long table_stride, const void* ids, int ids_are_64, void* out, int dtype, long n, long rows,
+                         int cols, float scale, void* stream);
+/* grad[r] = scale * sum of dout[t] over the tokens t with ids[t] == r; every row of grad [rows, cols] is written (0 without tokens),
+ * rows of dout whose id lies outside [0, rows) are not used.  grad_dtype: dtype or NS_F32.  The tokens are sorted by id on the device
+ * and the sums run over the sorted list in a fixed order: the same inputs give the same bits.
+ *   ws: ns_embedding_backward_workspace_bytes(n, rows, cols) bytes, 16-byte aligned, contents irrelevant; calls that may be in flight
+ *   at the same time must not share it.                                                                                        */
+size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols);
+int ns_embedding_backward(const void* dout, long dout_stride, int dtype, const void* ids, int ids_are_64, void* grad, int grad_dtype,
+                          long n, long rows, int cols, float scale, void* ws, size_t ws_bytes, void* stream);
+
+/* y = (x - mean) * rstd * weight + bias over the cols of every row (biased variance, rstd = 1 / sqrt(var + eps)); weight / bias [cols]
+ * of wdtype (dtype or NS_F32), each may be NULL; mean / rstd f32 [n], both or neither.  cols <= 16384.                          */
+int ns_layer_norm_forward(const void* x, long x_stride, const void* weight, const void* bias, int wdtype, void* y, float* mean,
+                          float* rstd, int dtype, long n, int cols, float eps, void* stream);
+/* With g = dy * weight and xh = (x - mean) * rstd:  dx = rstd * (g - mean(g) - xh * mean(g xh)), dweight = sum over rows of dy xh,
+ * dbias = sum over rows of dy (both of wdtype, in a fixed order).  weight, dweight and dbias: all or none (none: dx alone).
+ *   ws: ns_layer_norm_backward_workspace_bytes(n, cols, dtype) bytes (none without a weight), as above.                        */
+size_t ns_layer_norm_backward_workspace_bytes(long n, int cols, int dtype);
+int ns_layer_norm_backward(const void* dy, long dy_stride, const void* x, long x_stride, const float* mean, const float* rstd,
+                           const void* weight, int wdtype, void* dx, void* dweight, void* dbias, int dtype, long n, int cols, void* ws,
+                           size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

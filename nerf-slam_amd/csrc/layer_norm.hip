@@ -1,0 +1,323 @@
+// layer_norm.hip -- layer norm over the channels of a row and its backward pass.
+//
+//   forward    mean = sum(x) / D, var = sum((x - mean)^2) / D, rstd = 1 / sqrt(var + eps), y = (x - mean) rstd w + b
+//   backward   g = dy w, xh = (x - mean) rstd:   dx = rstd (g - sum(g) / D - xh sum(g xh) / D),   dw = sum over rows of dy xh,
+//              db = sum over rows of dy
+//
+// Bound by HBM: x in, y out (forward); x and dy in, dx out (backward).  A row is read ONCE and stays in registers between its sums and
+// its output: LPR lanes hold NV pieces of 16 bytes each.  The backward pass keeps the two weight gradients of its lanes' columns in f32
+// registers over all the rows that a workgroup takes, so they cost one partial row pair per workgroup and a second, small launch that
+// adds those in a fixed order: no atomics, the same bits on every run.  All sums are f32; every output is rounded once.
+#include "rows.h"
+
+#define LN_MAX_COLS 16384
+
+// sum over the LPR lanes of a row, LPR <= 64: every lane gets it.  DPP adds within 16 lanes (common.h), two exchanges beyond.
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if (LPR >= 2) v = dpp_add<0xB1, 0xf>(v);
+  if (LPR >= 4) v = dpp_add<0x4E, 0xf>(v);
+  if (LPR >= 8) v = dpp_add<0x141, 0xf>(v);
+  if (LPR >= 16) v = dpp_add<0x140, 0xf>(v);
+  if (LPR >= 32) v += __shfl_xor(v, 16, 64);
+  if (LPR >= 64) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+
+// two sums over the lanes of a row.  LPR > 64: the workgroup's waves meet in LDS; callers use two buffers in turn, so that one barrier
+// per call is enough (a wave writes a buffer again only behind the barrier of the call in between).
+template <int LPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2]) {
+  a = lanes_sum<(LPR < 64 ? LPR : 64)>(a);
+  b = lanes_sum<(LPR < 64 ? LPR : 64)>(b);
+  if (LPR > 64) {
+    constexpr int W = LPR / 64;
+    if ((threadIdx.x & 63) == 0) {
+      red[threadIdx.x >> 6][0] = a;
+      red[threadIdx.x >> 6][1] = b;
+    }
+    lds_barrier();
+    a = b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      a += red[i][0];
+      b += red[i][1];
+    }
+  }
+}
+
+template <int LPR>
+constexpr int ln_block() { return LPR > 256 ? LPR : 256; }
+
+// ---------------------------------------------------------------------------------------------
+// forward.  Two sums over the row, in turn: the mean, then sum d and sum d^2 of the deviations d = x - mean.  The first of these is what
+// rounding left of the mean; taking it out again keeps the deviations exact where |mean| is far above the row's spread.
+// ---------------------------------------------------------------------------------------------
+template <typename T, typename W, int LPR, int NV>
+__global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T* __restrict__ x, long xstride, const W* __restrict__ w,
+                                                                         const W* __restrict__ b, T* __restrict__ y,
+                                                                         float* __restrict__ mean, float* __restrict__ rstd, long n, int D,
+                                                                         float inv_d, float eps) {
+  constexpr int V = row_vec<T>(), ROWS = ln_block<LPR>() / LPR;
+  __shared__ float red[2][LPR > 64 ? LPR / 64 : 1][2];   // (per sum: the other sum's barrier lies between two uses)
+  const int lane = threadIdx.x % LPR;
+  const long step = (long)gridDim.x * ROWS;
+  RowPiece<W, V> wp[NV], bp[NV];
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const int c = (j * LPR + lane) * V;
+    if (w) wp[j] = row_load<W, V>(w, c, D);
+    if (b) bp[j] = row_load<W, V>(b, c, D);
+  }
+  for (long r = (long)blockIdx.x * ROWS + threadIdx.x / LPR; r < n; r += step) {
+    RowPiece<T, V> p[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) p[j] = row_load<T, V>(x + r * xstride, (j * LPR + lane) * V, D);
+    float f[NV][V], s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        f[j][i] = (float)p[j].e[i];
+        s += f[j][i];
+      }
+    row_sum2<LPR>(s, q, red[0]);
+    const float m1 = s * inv_d;
+    s = q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        f[j][i] = (j * LPR + lane) * V + i < D ? f[j][i] - m1 : 0.0f;
+        s += f[j][i];
+        q += f[j][i] * f[j][i];
+      }
+    row_sum2<LPR>(s, q, red[1]);
+    const float m2 = s * inv_d, var = fmaxf(q * inv_d - m2 * m2, 0.0f), rs = 1.0f / sqrtf(var + eps);
+    if (lane == 0 && mean) {
+      mean[r] = m1 + m2;
+      rstd[r] = rs;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        float v = (f[j][i] - m2) * rs;
+        if (w) v *= (float)wp[j].e[i];
+        if (b) v += (float)bp[j].e[i];
+        f[j][i] = v;
+      }
+      row_store<T, V>(y + r * D, (j * LPR + lane) * V, D, f[j]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// backward.  part: [workgroups][2][D] f32 (dw | db), or nullptr: no weight.
+// ---------------------------------------------------------------------------------------------
+template <typename T, typename W, int LPR, int NV>
+__global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T* __restrict__ dy, long dstride, const T* __restrict__ x,
+                                                                         long xstride, const float* __restrict__ mean,
+                                                                         const float* __restrict__ rstd, const W* __restrict__ w,
+                                                                         T* __restrict__ dx, float* __restrict__ part, long n, int D,
+                                                                         float inv_d) {
+  constexpr int V = row_vec<T>(), BLOCK = ln_block<LPR>(), ROWS = BLOCK / LPR;
+  __shared__ float red[2][LPR > 64 ? LPR / 64 : 1][2];
+  __shared__ float cols[ROWS > 1 ? BLOCK * (V + 1) : 1];
+  const int lane = threadIdx.x % LPR;
+  const long step = (long)gridDim.x * ROWS;
+  RowPiece<W, V> wp[NV];
+  float dw[NV][V], db[NV][V];
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    if (w) wp[j] = row_load<W, V>(w, (j * LPR + lane) * V, D);
+#pragma unroll
+    for (int i = 0; i < V; i++) dw[j][i] = db[j][i] = 0.0f;
+  }
+  int turn = 0;
+  for (long r = (long)blockIdx.x * ROWS + threadIdx.x / LPR; r < n; r += step, turn ^= 1) {
+    RowPiece<T, V> p[NV], d[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      p[j] = row_load<T, V>(x + r * xstride, (j * LPR + lane) * V, D);
+      d[j] = row_load<T, V>(dy + r * dstride, (j * LPR + lane) * V, D);
+    }
+    const float mu = mean[r], rs = rstd[r];
+    float s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const float u = (float)d[j].e[i];                       // (0 behind the end of the row, so g and both gradients are)
+        const float h = ((float)p[j].e[i] - mu) * rs, g = w ? u * (float)wp[j].e[i] : u;
+        db[j][i] += u;
+        dw[j][i] += u * h;
+        s += g;
+        q += g * h;
+      }
+    row_sum2<LPR>(s, q, red[turn]);
+    const float a = s * inv_d, b = q * inv_d;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      row_pin(p[j]);                                            // g and xh are formed again from the 16-byte pieces: held over the sums
+      row_pin(d[j]);                                            // they would take four times the registers
+      float f[V];
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const float u = (float)d[j].e[i], h = ((float)p[j].e[i] - mu) * rs, g = w ? u * (float)wp[j].e[i] : u;
+        f[i] = (g - a - h * b) * rs;
+      }
+      row_store<T, V>(dx + r * D, (j * LPR + lane) * V, D, f);
+    }
+  }
+  if (!part) return;
+  float* mine = part + (long)blockIdx.x * 2 * D;
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      float(&acc)[V] = k ? db[j] : dw[j];
+      if (ROWS > 1) {                                            // the workgroup's rows meet in LDS
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; i++) cols[threadIdx.x * (V + 1) + i] = acc[i];
+        __syncthreads();
+        if (threadIdx.x < LPR) {
+#pragma unroll
+          for (int t = 1; t < ROWS; t++)
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] += cols[(t * LPR + lane) * (V + 1) + i];
+        }
+      }
+      if (threadIdx.x < LPR) row_store<float, V>(mine + (long)k * D, (j * LPR + lane) * V, D, acc);
+    }
+}
+
+// dw | db [2 D] from the workgroups' partial rows: 64 columns per workgroup, 16 waves share the rows and meet in LDS
+template <typename W>
+__global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __restrict__ part, int parts, int D, W* __restrict__ dw,
+                                                                W* __restrict__ db) {
+  __shared__ float red[16][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float s = 0.0f;
+  if (c < 2 * D) {
+#pragma unroll 8
+    for (int i = wv; i < parts; i += 16) s += part[(long)i * 2 * D + c];
+  }
+  red[wv][lane] = s;
+  __syncthreads();
+  if (wv == 0 && c < 2 * D) {
+#pragma unroll
+    for (int i = 1; i < 16; i++) s += red[i][lane];
+    if (c < D) dw[c] = (W)s;
+    else db[c - D] = (W)s;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// C ABI
+// ---------------------------------------------------------------------------------------------
+// Calls f(LPR, NV) with the lanes per row and pieces per lane of a row of D elements.  Up to 128 pieces a wave (or less) holds a row
+// and no barrier is needed; beyond, four waves; beyond 1024 pieces, sixteen.
+template <int N>
+struct LnInt { static constexpr int v = N; };
+
+template <int V, typename F>
+static void ln_shape(int D, F f) {
+  const int pieces = (D + V - 1) / V;
+  if (pieces <= 8) f(LnInt<8>(), LnInt<1>());
+  else if (pieces <= 16) f(LnInt<16>(), LnInt<1>());
+  else if (pieces <= 32) f(LnInt<32>(), LnInt<1>());
+  else if (pieces <= 64) f(LnInt<64>(), LnInt<1>());
+  else if (pieces <= 128) f(LnInt<64>(), LnInt<2>());
+  else if (pieces <= 256) f(LnInt<256>(), LnInt<1>());
+  else if (pieces <= 512) f(LnInt<256>(), LnInt<2>());
+  else if (pieces <= 1024) f(LnInt<256>(), LnInt<4>());
+  else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
+  else if constexpr (V == 4) f(LnInt<1024>(), LnInt<4>());
+}
+
+// calls f(element, weight element) for a pair of dtypes; false: not a pair that the kernels have
+template <typename F>
+static bool ln_types(int dtype, int wdtype, F f) {
+  if (dtype == NS_F32 && wdtype == NS_F32) f(0.0f, 0.0f);
+  else if (dtype == NS_F16 && wdtype == NS_F16) f((_Float16)0, (_Float16)0);
+  else if (dtype == NS_F16 && wdtype == NS_F32) f((_Float16)0, 0.0f);
+  else if (dtype == NS_BF16 && wdtype == NS_BF16) f((rw_bf16)0.0f, (rw_bf16)0.0f);
+  else if (dtype == NS_BF16 && wdtype == NS_F32) f((rw_bf16)0.0f, 0.0f);
+  else return false;
+  return true;
+}
+
+static int ln_rows_per_block(int D, int vec) {
+  const int pieces = (D + vec - 1) / vec;
+  return pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 128 ? 4 : 1;
+}
+
+#define LN_FWD_BLOCKS 4096
+#define LN_BWD_BLOCKS 512
+
+static int ln_blocks(long n, int D, int dtype, int most) {
+  const int per = ln_rows_per_block(D, dtype == NS_F32 ? 4 : 8);
+  const long want = (n + per - 1) / per;
+  return (int)(want < most ? want : most);
+}
+
+extern "C" int ns_layer_norm_forward(const void* x, long x_stride, const void* weight, const void* bias, int wdtype, void* y, float* mean,
+                                     float* rstd, int dtype, long n, int cols, float eps, void* stream) {
+  NS_REQUIRE(n >= 0 && n <= (1L << 40) && cols >= 1 && cols <= LN_MAX_COLS && x_stride >= 0,
+             "ns_layer_norm_forward: bad shape (n %ld, cols %d in 1 .. %d)", n, cols, LN_MAX_COLS);
+  NS_REQUIRE(eps > 0.0f && eps < __builtin_inff(), "ns_layer_norm_forward: eps %g has to be positive and finite", (double)eps);
+  NS_REQUIRE((mean == nullptr) == (rstd == nullptr), "ns_layer_norm_forward: mean and rstd come together");
+  if (n == 0) return NS_OK;
+  NS_REQUIRE(x && y, "ns_layer_norm_forward: null pointer");
+  const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
+    using T = decltype(t);
+    using W = decltype(u);
+    ln_shape<row_vec<T>()>(cols, [&](auto lpr, auto nv) {
+      constexpr int L = decltype(lpr)::v, N = decltype(nv)::v;
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, L, N>), dim3(ln_blocks(n, cols, dtype, LN_FWD_BLOCKS)), dim3(ln_block<L>()), 0,
+                         (hipStream_t)stream, (const T*)x, x_stride, (const W*)weight, (const W*)bias, (T*)y, mean, rstd, n, cols,
+                         1.0f / (float)cols, eps);
+    });
+  });
+  NS_REQUIRE(ok, "ns_layer_norm_forward: dtype %d / weight dtype %d: NS_F16, NS_BF16 or NS_F32, weights the same or NS_F32", dtype, wdtype);
+  NS_CHECK_LAUNCH("layer_norm_fwd_kernel");
+  return NS_OK;
+}
+
+extern "C" size_t ns_layer_norm_backward_workspace_bytes(long n, int cols, int dtype) {
+  if (n <= 0 || cols < 1 || cols > LN_MAX_COLS) return 0;
+  return (size_t)ln_blocks(n, cols, dtype, LN_BWD_BLOCKS) * 2 * cols * 4;
+}
+
+extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void* x, long x_stride, const float* mean, const float* rstd,
+                                      const void* weight, int wdtype, void* dx, void* dweight, void* dbias, int dtype, long n, int cols,
+                                      void* ws, size_t ws_bytes, void* stream) {
+  NS_REQUIRE(n >= 0 && n <= (1L << 40) && cols >= 1 && cols <= LN_MAX_COLS && x_stride >= 0 && dy_stride >= 0,
+             "ns_layer_norm_backward: bad shape (n %ld, cols %d in 1 .. %d)", n, cols, LN_MAX_COLS);
+  NS_REQUIRE(n == 0 || (dy && x && mean && rstd && dx), "ns_layer_norm_backward: null pointer");
+  NS_REQUIRE((weight != nullptr) == (dweight != nullptr) && (weight != nullptr) == (dbias != nullptr),
+             "ns_layer_norm_backward: weight, dweight and dbias come together");
+  const size_t need = weight ? ns_layer_norm_backward_workspace_bytes(n, cols, dtype) : 0;
+  NS_REQUIRE(ws_bytes >= need && (ws || need == 0), "ns_layer_norm_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  const int blocks = ln_blocks(n, cols, dtype, LN_BWD_BLOCKS);
+  const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
+    using T = decltype(t);
+    using W = decltype(u);
+    if (n > 0)
+      ln_shape<row_vec<T>()>(cols, [&](auto lpr, auto nv) {
+        constexpr int L = decltype(lpr)::v, N = decltype(nv)::v;
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, L, N>), dim3(blocks), dim3(ln_block<L>()), 0, (hipStream_t)stream, (const T*)dy,
+                           dy_stride, (const T*)x, x_stride, mean, rstd, (const W*)weight, (T*)dx, weight ? (float*)ws : nullptr, n, cols,
+                           1.0f / (float)cols);
+      });
+    if (weight)
+      hipLaunchKernelGGL(layer_norm_wgrad_kernel<W>, dim3((2 * cols + 63) / 64), dim3(1024), 0, (hipStream_t)stream, (const float*)ws, blocks,
+                         cols, (W*)dweight, (W*)dbias);
+  });
+  NS_REQUIRE(ok, "ns_layer_norm_backward: dtype %d / weight dtype %d: NS_F16, NS_BF16 or NS_F32, weights the same or NS_F32", dtype, wdtype);
+  NS_CHECK_LAUNCH("layer_norm_bwd_kernel");
+  return NS_OK;
+}

@@ -1,0 +1,62 @@
+// rows.h -- pieces shared by the row operators (embedding.hip, layer_norm.hip): a row of features is D elements of f16, bf16 or f32
+// that follow each other in memory; rows are `stride` elements apart.  Every lane moves 16 bytes of a row at a time.
+#pragma once
+#include "common.h"
+
+typedef __bf16 rw_bf16;
+
+// elements of T in 16 bytes: what a lane holds of a row
+template <typename T>
+constexpr int row_vec() { return 16 / (int)sizeof(T); }
+
+// N elements of T as they lie in memory.  Loads and stores go through memcpy, so that they only assume the alignment of an element:
+// gfx950 takes 16-byte accesses at any address, and rows of an odd length need no kernel of their own.
+template <typename T, int N>
+struct RowPiece {
+  T e[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ RowPiece<T, N> row_load(const T* __restrict__ row, int c, int D) {
+  RowPiece<T, N> v;
+  if (c + N <= D) {
+    __builtin_memcpy(&v, row + c, sizeof(v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v.e[i] = c + i < D ? row[c + i] : (T)0.0f;
+  }
+  return v;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void row_store(T* __restrict__ row, int c, int D, const float* f) {
+  RowPiece<T, N> v;
+#pragma unroll
+  for (int i = 0; i < N; i++) v.e[i] = (T)f[i];      // one rounding, to nearest even
+  if (c + N <= D) {
+    __builtin_memcpy(row + c, &v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (c + i < D) row[c + i] = v.e[i];
+  }
+}
+
+// the 16 bytes become opaque to the compiler: what is computed from them again is not kept from the first time
+template <typename T, int N>
+__device__ __forceinline__ void row_pin(RowPiece<T, N>& v) {
+  typedef int v4i __attribute__((ext_vector_type(4)));
+  static_assert(sizeof(v) == sizeof(v4i), "a 16-byte piece");
+  v4i q;
+  __builtin_memcpy(&q, &v, sizeof(q));
+  asm volatile("" : "+v"(q));
+  __builtin_memcpy(&v, &q, sizeof(q));
+}
+
+// lanes that share a row: the power of two that covers its 16-byte pieces, at least 1, at most 64
+static inline int row_lanes_log2(int D, int vec) {
+  const int pieces = (D + vec - 1) / vec;
+  int s = 0;
+  while (s < 6 && (1 << s) < pieces) s++;
+  return s;
+}

@@ -49,6 +49,8 @@ def _load(path):
     L.ns_ngp_encode_backward_fused_workspace_bytes.restype = C.c_size_t
     L.ns_ba_solve_large_workspace_bytes.restype = C.c_size_t
     L.ns_ngp_mlp_fragment_table_bytes.restype = C.c_size_t
+    L.ns_embedding_backward_workspace_bytes.restype = C.c_size_t
+    L.ns_layer_norm_backward_workspace_bytes.restype = C.c_size_t
     return L
 
 

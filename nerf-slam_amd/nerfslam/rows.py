@@ -1,0 +1,166 @@
+"""Operators on rows of features: a table looked up by id (a latent per keyframe, a vector per token) with the table's gradient, and
+layer norm over a row with its backward pass -- host side of `csrc/embedding.hip` and `csrc/layer_norm.hip`.
+
+A row is the last axis of a tensor (f16, bf16 or f32): channels-last activations as `nerfslam.conv` keeps them are rows of C channels.
+Inputs may be slices of wider tensors or expanded along the leading axes, as long as the last axis is dense and the leading ones
+collapse to one stride; outputs are fresh dense tensors.  Sums are f32, every output is rounded once.  The backward functions are
+explicit, as the trainer's are: nothing here records on torch's autograd tape.  Launches go to torch's current stream of the tensors'
+device, nothing synchronises, and every call has its own workspace, so calls may be captured into HIP graphs and run on several streams.
+"""
+import ctypes as C
+
+import torch
+
+from ._lib import NerfSlamHipError, check, lib, ptr, require_cuda, stream_ptr
+
+_DT = {torch.float16: 1, torch.float32: 2, torch.bfloat16: 3}
+
+
+def _fail(op, what):
+    raise NerfSlamHipError(f"{op}: {what}")
+
+
+def _same_device(op, *tensors):
+    require_cuda(*tensors)
+    if len({t.device for t in tensors if t is not None}) > 1:
+        _fail(op, "all tensors have to be on one device")
+
+
+def _rows_of(op, name, t):
+    """(number of rows, distance of two rows in elements) of a tensor whose last axis is the row"""
+    if t.dtype not in _DT:
+        _fail(op, f"{name} is {t.dtype}: float16, bfloat16 or float32 are supported")
+    if t.dim() < 1:
+        _fail(op, f"{name} needs at least one axis")
+    cols, n = int(t.shape[-1]), 1
+    for s in t.shape[:-1]:
+        n *= int(s)
+    if n * cols == 0:
+        return n, cols
+    if cols > 1 and t.stride(-1) != 1:
+        _fail(op, f"the last axis of {name} must be contiguous")
+    stride, inner = None, 1                 # collapse the leading axes, innermost first; axes of size 1 have no stride to mind
+    for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if stride is None:
+            stride = int(st)
+        elif int(st) != stride * inner:
+            _fail(op, f"the rows of {name} are not a constant stride apart: pass {name}.contiguous()")
+        inner *= int(size)
+    return n, cols if stride is None else stride
+
+
+def _ids(op, ids):
+    if ids.dtype not in (torch.int32, torch.int64):
+        _fail(op, f"ids are {ids.dtype}: int32 or int64 are supported")
+    if not ids.is_contiguous():
+        raise RuntimeError("ids must be contiguous")
+    return int(ids.dtype == torch.int64)
+
+
+def embedding(table, ids, scale=1.0):
+    """table [rows, D], ids (any shape, int32 / int64) -> ids.shape + (D,) in the table's dtype: scale * table[ids].  An id outside
+    [0, rows), e.g. -1 for a padded place, gives a row of zeros."""
+    if table.dim() != 2:
+        _fail("embedding", "the table is a [rows, D] tensor")
+    rows, stride = _rows_of("embedding", "table", table)
+    is64 = _ids("embedding", ids)
+    _same_device("embedding", table, ids)
+    out = torch.empty((*ids.shape, table.shape[1]), dtype=table.dtype, device=table.device)
+    if out.numel() == 0:
+        return out
+    with torch.cuda.device(out.device):
+        check(lib().ns_embedding_forward(ptr(table), C.c_long(stride), ptr(ids), is64, ptr(out), _DT[table.dtype], C.c_long(ids.numel()),
+                                         C.c_long(rows), int(table.shape[1]), C.c_float(scale), stream_ptr()), "embedding_forward")
+    return out
+
+
+def embedding_backward(dout, ids, rows, scale=1.0, dtype=None):
+    """gradient of `embedding` for its table: dout ids.shape + (D,) -> [rows, D] of `dtype` (None: float32; or dout's own),
+    grad[r] = scale * sum of dout over the places with id r; zero where there is none.  Places whose id is outside [0, rows) are left
+    out.  The order of the sums follows from the ids alone: the same inputs give the same bits."""
+    op = "embedding_backward"
+    dtype = torch.float32 if dtype is None else dtype
+    if dout.dim() != ids.dim() + 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
+        _fail(op, f"dout {tuple(dout.shape)} does not match ids {tuple(ids.shape)} + (D,)")
+    n, stride = _rows_of(op, "dout", dout)
+    if dtype not in (torch.float32, dout.dtype):
+        _fail(op, f"a gradient in {dtype} of a {dout.dtype} dout: float32 or dout's own dtype are supported")
+    is64 = _ids(op, ids)
+    rows, cols = int(rows), int(dout.shape[-1])
+    if rows < 0:
+        _fail(op, f"{rows} rows")
+    _same_device(op, dout, ids)
+    grad = torch.empty((rows, cols), dtype=dtype, device=dout.device)
+    if grad.numel() == 0:
+        return grad
+    with torch.cuda.device(grad.device):
+        nbytes = int(lib().ns_embedding_backward_workspace_bytes(C.c_long(n), C.c_long(rows), cols))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
+        check(lib().ns_embedding_backward(ptr(dout), C.c_long(stride), _DT[dout.dtype], ptr(ids), is64, ptr(grad), _DT[dtype], C.c_long(n),
+                                          C.c_long(rows), cols, C.c_float(scale), ptr(ws), C.c_size_t(nbytes), stream_ptr()), op)
+    return grad
+
+
+def _weights(op, x, **named):
+    """the common dtype of the weights that are there (x's own or float32); None: there are none"""
+    dtype = None
+    for name, t in named.items():
+        if t is None:
+            continue
+        if t.dtype not in (x.dtype, torch.float32):
+            _fail(op, f"{name} is {t.dtype}: {x.dtype} (as x) or float32 are supported")
+        if tuple(t.shape) != (int(x.shape[-1]),) or not t.is_contiguous():
+            _fail(op, f"{name} must be a contiguous [{int(x.shape[-1])}] tensor")
+        if dtype is not None and t.dtype != dtype:
+            _fail(op, "weight and bias have to be of one dtype")
+        dtype = t.dtype
+    return dtype
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=False):
+    """(x - mean) * rstd * weight + bias over the last axis (at most 16384 wide), rstd = 1 / sqrt(var + eps) with the biased variance;
+    weight / bias [D] in x's dtype or float32, each may be None.  stats=True: (y, mean, rstd), the latter two float32 of x.shape[:-1] --
+    what `layer_norm_backward` takes."""
+    op = "layer_norm"
+    n, stride = _rows_of(op, "x", x)
+    wdtype = _weights(op, x, weight=weight, bias=bias) or torch.float32
+    _same_device(op, x, weight, bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    with torch.cuda.device(x.device):
+        check(lib().ns_layer_norm_forward(ptr(x), C.c_long(stride), ptr(weight), ptr(bias), _DT[wdtype], ptr(y), ptr(mean), ptr(rstd),
+                                          _DT[x.dtype], C.c_long(n), int(x.shape[-1]), C.c_float(eps), stream_ptr()), "layer_norm_forward")
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm_backward(dout, x, mean, rstd, weight=None):
+    """gradients of `layer_norm` from the upstream gradient dout (x's shape and dtype) and what the forward pass saved:
+    (dx, dweight, dbias) -- dx in x's dtype, the other two in the weight's; (dx, None, None) without a weight."""
+    op = "layer_norm_backward"
+    n, stride = _rows_of(op, "x", x)
+    if dout.dtype != x.dtype or tuple(dout.shape) != tuple(x.shape):
+        _fail(op, f"dout {tuple(dout.shape)} {dout.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    _, dstride = _rows_of(op, "dout", dout)
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.dtype != torch.float32 or tuple(t.shape) != tuple(x.shape[:-1]) or not t.is_contiguous():
+            _fail(op, f"{name} must be a contiguous float32 {tuple(x.shape[:-1])} tensor")
+    wdtype = _weights(op, x, weight=weight) or torch.float32
+    _same_device(op, x, dout, mean, rstd, weight)
+    cols = int(x.shape[-1])
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = db = ws = None
+    nbytes = 0
+    if weight is not None:
+        dw, db = torch.empty_like(weight), torch.empty_like(weight)
+    with torch.cuda.device(x.device):
+        if weight is not None:
+            nbytes = int(lib().ns_layer_norm_backward_workspace_bytes(C.c_long(n), cols, _DT[x.dtype]))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        check(lib().ns_layer_norm_backward(ptr(dout), C.c_long(dstride), ptr(x), C.c_long(stride), ptr(mean), ptr(rstd), ptr(weight), _DT[wdtype],
+                                           ptr(dx), ptr(dw), ptr(db), _DT[x.dtype], C.c_long(n), cols, ptr(ws), C.c_size_t(nbytes),
+                                           stream_ptr()), op)
+    return dx, dw, db
