@@ -753,9 +753,9 @@ int ns_embedding_forward(const void* table, long table_stride, const void* ids, 
 /* grad[r] = scale * sum of dout[t] over the tokens t with ids[t] == r; every row of grad [rows, cols] is written (0 without tokens),
  * rows of dout whose id lies outside [0, rows) are not used.  grad_dtype: dtype or NS_F32.  The tokens are sorted by id on the device
  * and the sums run over the sorted list in a fixed order: the same inputs give the same bits.
- *   ws: ns_embedding_backward_workspace_bytes(n, rows, cols) bytes, 16-byte aligned, contents irrelevant; calls that may be in flight
+ *   ws: ns_embedding_backward_workspace_bytes(n, rows, cols, dtype) bytes, 16-byte aligned, contents irrelevant; calls that may be in flight
  *   at the same time must not share it.                                                                                        */
-size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols);
+size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols, int dtype);
 int ns_embedding_backward(const void* dout, long dout_stride, int dtype, const void* ids, int ids_are_64, void* grad, int grad_dtype,
                           long n, long rows, int cols, float scale, void* ws, size_t ws_bytes, void* stream);
 

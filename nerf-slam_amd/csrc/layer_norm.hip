@@ -46,6 +46,11 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2]) {
   }
 }
 
+#ifdef LN512
+#define LNX LnInt<512>(), LnInt<2>()
+#else
+#define LNX LnInt<256>(), LnInt<4>()
+#endif
 template <int LPR>
 constexpr int ln_block() { return LPR > 256 ? LPR : 256; }
 
@@ -134,15 +139,34 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
 #pragma unroll
     for (int i = 0; i < V; i++) dw[j][i] = db[j][i] = 0.0f;
   }
-  int turn = 0;
-  for (long r = (long)blockIdx.x * ROWS + threadIdx.x / LPR; r < n; r += step, turn ^= 1) {
+  // the next row is on its way while this one is worked on, where the registers allow it
+  #ifndef LNAHEAD
+#define LNAHEAD (LPR < 1024 && NV < 4)
+#endif
+  constexpr bool AHEAD = LNAHEAD;
+  RowPiece<T, V> pn[NV], dn[NV];
+  float mun = 0.0f, rsn = 0.0f;
+  auto fetch = [&](long r) {
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      pn[j] = row_load<T, V>(x + r * xstride, (j * LPR + lane) * V, D);
+      dn[j] = row_load<T, V>(dy + r * dstride, (j * LPR + lane) * V, D);
+    }
+    mun = mean[r];
+    rsn = rstd[r];
+  };
+  long r = (long)blockIdx.x * ROWS + threadIdx.x / LPR;
+  if (AHEAD && r < n) fetch(r);
+  for (int turn = 0; r < n; r += step, turn ^= 1) {
+    if (!AHEAD) fetch(r);
     RowPiece<T, V> p[NV], d[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      p[j] = row_load<T, V>(x + r * xstride, (j * LPR + lane) * V, D);
-      d[j] = row_load<T, V>(dy + r * dstride, (j * LPR + lane) * V, D);
+      p[j] = pn[j];
+      d[j] = dn[j];
     }
-    const float mu = mean[r], rs = rstd[r];
+    const float mu = mun, rs = rsn;
+    if (AHEAD && r + step < n) fetch(r + step);
     float s = 0.0f, q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; j++)
@@ -233,7 +257,7 @@ static void ln_shape(int D, F f) {
   else if (pieces <= 128) f(LnInt<64>(), LnInt<2>());
   else if (pieces <= 256) f(LnInt<256>(), LnInt<1>());
   else if (pieces <= 512) f(LnInt<256>(), LnInt<2>());
-  else if (pieces <= 1024) f(LnInt<256>(), LnInt<4>());
+  else if (pieces <= 1024) f(LNX);
   else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
   else if constexpr (V == 4) f(LnInt<1024>(), LnInt<4>());
 }
@@ -255,8 +279,12 @@ static int ln_rows_per_block(int D, int vec) {
   return pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 128 ? 4 : 1;
 }
 
+#ifndef LN_FWD_BLOCKS
 #define LN_FWD_BLOCKS 4096
+#endif
+#ifndef LN_BWD_BLOCKS
 #define LN_BWD_BLOCKS 512
+#endif
 
 static int ln_blocks(long n, int D, int dtype, int most) {
   const int per = ln_rows_per_block(D, dtype == NS_F32 ? 4 : 8);

@@ -484,7 +484,7 @@ def test_nothing_is_written_outside_the_outputs(dev):
         _, p, inner, ok = room(n * d, F16)
         check(f.ns_embedding_forward(ptr(table), L(d), ptr(ids), 0, p, 1, L(n), L(v), d, C.c_float(1), stream_ptr()), "fwd")
         assert ok() and torch.equal(inner().view(n, d), rows.embedding(table.view(v, d), ids))
-        need = f.ns_embedding_backward_workspace_bytes(L(n), L(v), d)
+        need = f.ns_embedding_backward_workspace_bytes(L(n), L(v), d, 1)
         ws = torch.full((need + 256,), 0x5a, dtype=torch.uint8, device=dev)
         _, p, inner, ok = room(v * d, F16)
         check(f.ns_embedding_backward(ptr(x), L(d), 1, ptr(ids), 0, p, 1, L(n), L(v), d, C.c_float(1), ptr(ws), C.c_size_t(need), stream_ptr()), "bwd")

@@ -107,8 +107,8 @@ def test_abi_refusals():
 def test_workspace_sizes():
     f = lib()
     emb, ln = f.ns_embedding_backward_workspace_bytes, f.ns_layer_norm_backward_workspace_bytes
-    assert emb(L(0), L(5), 4) == 0 and ln(L(0), 4, 2) == 0
+    assert emb(L(0), L(5), 4, 1) == 0 and ln(L(0), 4, 2) == 0
     for n in (1, 17, 8192, 8193, 1 << 20):
-        assert emb(L(n), L(1000), 64) >= 8 * n and emb(L(n), L(1000), 64) % 16 == 0
-    assert emb(L(1 << 27), L(1 << 29), 8) > 2 ** 31          # (no 32-bit arithmetic in it)
+        assert emb(L(n), L(1000), 64, 2) >= 8 * n and emb(L(n), L(1000), 64, 3) % 16 == 0
+    assert emb(L(1 << 27), L(1 << 29), 8, 1) > 2 ** 31          # (no 32-bit arithmetic in it)
     assert ln(L(10), 64, 2) % 512 == 0 and ln(L(1 << 20), 64, 2) > 0
