@@ -747,7 +747,7 @@ int ns_ngp_grid_update_sampled(const void* net_out, const int* cells, int n, flo
  * ---------------------------------------------------------------------------------------- */
 
 /* out[t] = scale * table[ids[t]]; an id outside [0, rows) (a padded place) gives a row of zeros.
- *   table [rows, cols] dtype, ids [n] int32 (int64 if ids_are_64), out [n, cols] dtype; n <= 2^27, rows <= 2^29, cols <= 65536. */
+ *   table [rows, cols] dtype, ids [n] int32 (int64 if ids_are_64), out [n, cols] dtype; n <= 2^25, rows <= 2^29, cols <= 65536. */
 int ns_embedding_forward(const void* table, long table_stride, const void* ids, int ids_are_64, void* out, int dtype, long n, long rows,
                          int cols, float scale, void* stream);
 /* grad[r] = scale * sum of dout[t] over the tokens t with ids[t] == r; every row of grad [rows, cols] is written (0 without tokens),

@@ -12,10 +12,12 @@
 //   2. sums   a group of lanes walks GROUP consecutive places and sums runs of equal ids in f32 registers; a run inside the share
 //             is final, a run that crosses its ends leaves one f32 partial row per share
 //   3. join   the share in which a crossing run begins adds its partial rows in order (embed_join_kernel)
+//
+// Columns: a lane holds V of them, 16 bytes, or one where a row is shorter than 16 bytes.  The last piece of a row ends with the row, so
+// where D is no multiple of V it overlaps the one before: both lanes form the same sums in the same order and store the same bits.
 #include "rows.h"
 
 #define RANK_MAX 8192        // tokens whose places are counted directly
-#define RANK_WAVES 16
 #ifndef ONE_MAX
 #define ONE_MAX 32768        // tokens up to which a radix pass is one launch
 #endif
@@ -27,129 +29,141 @@
 #define GROUP_WAVES 2048
 #endif
 #ifndef ZERO_ROWS
-#define ZERO_ROWS 32         // table rows per wave that looks for rows without tokens
+#define ZERO_ROWS 8         // table rows per wave that looks for rows without tokens
 #endif
-#ifndef EMB_U
-#define EMB_U 4
+#ifndef SUM_U
+#define SUM_U 8
 #endif
-#define MAX_BINS 1024
+#define MAX_BITS 10          // of a radix pass' digit
+#define MAX_BINS (1 << MAX_BITS)
+#ifndef FEW_ROWS
+#define FEW_ROWS (MAX_BINS - 1)
+#endif
+#ifndef FEW_LANES
+#define FEW_LANES 3
+#endif
+#define FEW_TILES 1024
 
-// ---------------------------------------------------------------------------------------------
-// forward: lanes (1 << ls) per token, EMB_U tokens per group so that their id -> row round trips overlap
-// ---------------------------------------------------------------------------------------------
 template <typename I>
-__device__ __forceinline__ unsigned emb_key(const I* __restrict__ ids, long t, unsigned rows) {
-  const I v = ids[t];
-  return v >= 0 && v < (I)rows ? (unsigned)v : rows;       // rows: the key of a padded place, sorted behind every row
+__device__ __forceinline__ unsigned emb_key(I id, unsigned rows) {
+  return id >= 0 && id < (I)rows ? (unsigned)id : rows;    // rows: the key of a padded place, sorted behind every row
 }
 
-template <typename T, typename I>
+// ---------------------------------------------------------------------------------------------
+// forward: (1 << ls) lanes per token
+// ---------------------------------------------------------------------------------------------
+template <typename T, int V, typename I>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ table, long tstride, const I* __restrict__ ids,
                                                         T* __restrict__ out, long n, unsigned rows, int D, int ls, float scale) {
-  constexpr int V = row_vec<T>();
-  const int lane = threadIdx.x & ((1 << ls) - 1), grp = threadIdx.x >> ls, step = 256 >> ls;
-  const long t0 = (long)blockIdx.x * (step * EMB_U) + grp;
-  unsigned key[EMB_U];
+  const int lane = threadIdx.x & ((1 << ls) - 1);
+  const long t = (long)blockIdx.x * (256 >> ls) + (threadIdx.x >> ls);
+  if (t >= n) return;
+  const unsigned key = emb_key(ids[t], rows);
+  const bool live = key < rows;
+  const T* row = table + (live ? (long)key * tstride : 0);
+  for (int p = lane * V; p < D; p += V << ls) {
+    const int c = min(p, D - V);
+    float f[V];
 #pragma unroll
-  for (int u = 0; u < EMB_U; u++) {
-    const long t = t0 + (long)u * step;
-    key[u] = t < n ? emb_key(ids, t, rows) : rows;
-  }
-  for (int c = lane * V; c < D; c += V << ls) {
-    RowPiece<T, V> v[EMB_U];
+    for (int i = 0; i < V; i++) f[i] = 0.0f;
+    if (live) {
+      const RowPiece<T, V> v = row_get<T, V>(row + c);
 #pragma unroll
-    for (int u = 0; u < EMB_U; u++) {
-      if (key[u] < rows) {
-        v[u] = row_load<T, V>(table + (long)key[u] * tstride, c, D);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) v[u].e[i] = (T)0.0f;
-      }
+      for (int i = 0; i < V; i++) f[i] = (float)v.e[i] * scale;
     }
-#pragma unroll
-    for (int u = 0; u < EMB_U; u++) {
-      const long t = t0 + (long)u * step;
-      float f[V];
-#pragma unroll
-      for (int i = 0; i < V; i++) f[i] = key[u] < rows ? (float)v[u].e[i] * scale : 0.0f;   // (0 * scale: also where scale is inf)
-      if (t < n) row_store<T, V, true>(out + t * D, c, D, f);
-    }
+    row_put<T, V, true>(out + t * D + c, f);
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// sort, short lists: the place of token t is the number of tokens with a smaller key, or the same key and a smaller index.  A
-// workgroup places 64 tokens (one per lane); its 16 waves share the list, which lies in LDS.  n^2 compares at 2 vector
-// instructions each.
+// sort, short lists: the place of token t is the number of tokens with a smaller key, or the same key and a smaller index: n^2 compares
+// at two vector instructions.  A workgroup places RANK_TOKENS tokens; its 16 waves, and the parts of a wave, each compare them with their
+// part of the list, which lies in LDS.
 // ---------------------------------------------------------------------------------------------
+#define RANK_WAVES 16
+#define RANK_TOKENS 16       // = RANK_WAVES: wave w compares the workgroup's tokens with its w-th
 template <typename I>
 __global__ __launch_bounds__(64 * RANK_WAVES) void embed_rank_kernel(const I* __restrict__ ids, int n, unsigned rows,
                                                                      unsigned* __restrict__ keys, int* __restrict__ order) {
+  constexpr int THREADS = 64 * RANK_WAVES, PARTS = THREADS / RANK_TOKENS;
   __shared__ __align__(16) unsigned k[RANK_MAX];
   __shared__ int cnt[RANK_WAVES][64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int n4 = (n + 3) & ~3;
-  for (int i = tid; i < n4; i += 64 * RANK_WAVES) k[i] = i < n ? emb_key(ids, i, rows) : 0xffffffffu;   // (sorted behind all)
+  I id[RANK_MAX / THREADS];
+#pragma unroll
+  for (int u = 0; u < RANK_MAX / THREADS; u++) id[u] = u * THREADS < n ? ids[min(u * THREADS + tid, n - 1)] : (I)0;
+#pragma unroll
+  for (int u = 0; u < RANK_MAX / THREADS; u++) {
+    const int i = u * THREADS + tid;
+    if (i < n4) k[i] = i < n ? emb_key(id[u], rows) : 0xffffffffu;       // (sorted behind all)
+  }
   __syncthreads();
-  const int b0 = blockIdx.x * 64, t = b0 + lane;
+  const int b0 = blockIdx.x * RANK_TOKENS, me = lane % RANK_TOKENS, t = b0 + me;
   const unsigned key = t < n ? k[t] : 0u;
-  const int per = ((n4 / 4 + RANK_WAVES - 1) / RANK_WAVES) * 4;
-  const int lo = min(w * per, n4), hi = min(lo + per, n4);
-  int c = 0;
-#pragma unroll 8
-  for (int i = lo; i < min(hi, b0); i += 4) {                     // before the 64 tokens: ties count
+  const int per = ((n4 / 4 + PARTS - 1) / PARTS) * 4;
+  const int lo = min((tid / RANK_TOKENS) * per, n4), hi = min(lo + per, n4);
+  unsigned c = 0;
+#pragma unroll 4
+  for (int i = lo; i < min(hi, b0); i += 4) {                     // before the workgroup's tokens: ties count
     const uint4 q = *reinterpret_cast<const uint4*>(&k[i]);
     c += (q.x <= key) + (q.y <= key) + (q.z <= key) + (q.w <= key);
   }
-#pragma unroll
-  for (int u = 0; u < 64 / RANK_WAVES; u++) {                     // among them (their keys are the lanes' own): ties with a smaller
-    const int i = w * (64 / RANK_WAVES) + u;                      // index count
-    const unsigned q = (unsigned)__builtin_amdgcn_readlane((int)key, i);
-    c += b0 + i < n && (q < key || (q == key && i < lane));
-  }
-#pragma unroll 8
-  for (int i = max(lo, b0 + 64); i < hi; i += 4) {                // behind them: ties do not count
+#pragma unroll 4
+  for (int i = max(lo, b0 + RANK_TOKENS); i < hi; i += 4) {       // behind them: ties do not count
     const uint4 q = *reinterpret_cast<const uint4*>(&k[i]);
     c += (q.x < key) + (q.y < key) + (q.z < key) + (q.w < key);
   }
-  cnt[w][lane] = c;
+  {                                                               // among them: ties with a smaller index count
+    const unsigned q = (unsigned)__builtin_amdgcn_readlane((int)key, w);
+    c += lane < RANK_TOKENS && b0 + w < n && (q < key || (q == key && w < me));
+  }
+  cnt[w][lane] = (int)c;
   __syncthreads();
-  if (w == 0 && t < n) {
+  if (w == 0) {
     int p = 0;
 #pragma unroll
     for (int i = 0; i < RANK_WAVES; i++) p += cnt[i][lane];
-    keys[p] = key;
-    order[p] = t;
+#pragma unroll
+    for (int o = RANK_TOKENS; o < 64; o <<= 1) p += __shfl_xor(p, o, 64);
+    if (lane < RANK_TOKENS && t < n) {
+      keys[p] = key;
+      order[p] = t;
+    }
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // sort, long lists: stable radix passes from the low digit up.  keys_in == nullptr: the first pass reads the ids.
 // ---------------------------------------------------------------------------------------------
+template <typename I>
+__device__ __forceinline__ unsigned emb_key_at(const I* __restrict__ ids, const unsigned* __restrict__ keys_in, long t, unsigned rows) {
+  return keys_in ? keys_in[t] : emb_key(ids[t], rows);
+}
+
 // Digits are counted in COPIES copies of the counters, by lane: where the same id fills a wave, its LDS atomics queue up a quarter as long.
 #define COPIES 4
 template <typename I>
 __global__ __launch_bounds__(256) void embed_hist_kernel(const I* __restrict__ ids, const unsigned* __restrict__ keys_in, long n,
-                                                         unsigned rows, int shift, int bins, int* __restrict__ hist) {
+                                                         unsigned rows, int shift, int bins, int used,
+                                                         int* __restrict__ hist) {
   __shared__ int h[COPIES * MAX_BINS];
   const int tid = threadIdx.x, copy = tid & (COPIES - 1);
   for (int i = tid; i < COPIES * bins; i += 256) h[i] = 0;
   __syncthreads();
-  const long t0 = (long)blockIdx.x * TILE;
+  const long t0 = (long)blockIdx.x * TILE + tid;
+  unsigned key[TILE / 256];
 #pragma unroll
-  for (int i = 0; i < TILE / 256; i++) {
-    const long t = t0 + i * 256 + tid;
-    if (t < n) {
-      const unsigned key = keys_in ? keys_in[t] : emb_key(ids, t, rows);
-      atomicAdd(&h[((key >> shift) & (bins - 1)) * COPIES + copy], 1);
-    }
-  }
+  for (int i = 0; i < TILE / 256; i++) key[i] = emb_key_at(ids, keys_in, min(t0 + i * 256, n - 1), rows);
+#pragma unroll
+  for (int i = 0; i < TILE / 256; i++)
+    if (t0 + i * 256 < n) atomicAdd(&h[((key[i] >> shift) & (bins - 1)) * COPIES + copy], 1);
   __syncthreads();
-  for (int i = tid; i < bins; i += 256) {
+  for (int i = tid; i < used; i += 256) {
     int c = 0;
 #pragma unroll
     for (int k = 0; k < COPIES; k++) c += h[i * COPIES + k];
-    hist[(long)blockIdx.x * bins + i] = c;
+    hist[(long)blockIdx.x * used + i] = c;
   }
 }
 
@@ -202,21 +216,36 @@ __device__ __forceinline__ unsigned long long emb_same_digit(int d, int bits, bo
 template <typename I>
 __global__ __launch_bounds__(256) void embed_scatter_kernel(const I* __restrict__ ids, const unsigned* __restrict__ keys_in,
                                                             const int* __restrict__ order_in, long n, unsigned rows, int shift,
-                                                            int bits, const int* __restrict__ hist, const int* __restrict__ total,
+                                                            int bits, int used, const int* __restrict__ hist,
+                                                            const int* __restrict__ total,
                                                             unsigned* __restrict__ keys_out, int* __restrict__ order_out) {
   __shared__ int off[4][MAX_BINS];
   __shared__ int part[4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int bins = 1 << bits, per = (bins + 255) / 256;
+  const int bins = 1 << bits;
   const long t0 = (long)blockIdx.x * TILE + w * (TILE / 4);
-  constexpr int STEPS = TILE / 256;
-  for (int i = tid; i < 4 * bins; i += 256) off[i >> bits][i & (bins - 1)] = 0;
-  // first place of every digit: prefix of the totals (thread: `per` neighbouring digits)
-  int sum = 0;
-  for (int i = 0; i < per; i++) {
-    const int d = tid * per + i;
-    sum += d < bins ? total[d] : 0;
+  constexpr int STEPS = TILE / 256, PER = MAX_BINS / 256;
+  // all loads first
+  unsigned key[STEPS];
+  int from[STEPS], tot[PER], before_tile[PER];
+#pragma unroll
+  for (int s = 0; s < STEPS; s++) {
+    const long t = min(t0 + s * 64 + lane, n - 1);
+    key[s] = emb_key_at(ids, keys_in, t, rows);
+    from[s] = order_in ? order_in[t] : (int)t;
   }
+  // (thread: PER neighbouring digits)
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const int d = tid * PER + i;
+    tot[i] = d < used ? total[d] : 0;
+    before_tile[i] = d < used ? hist[(long)blockIdx.x * used + d] : 0;
+  }
+  for (int i = tid; i < 4 * bins; i += 256) off[i >> bits][i & (bins - 1)] = 0;
+  // first place of every digit: prefix of the totals
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) sum += tot[i];
   int upto = sum;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -225,13 +254,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I* __restrict_
   }
   if (lane == 63) part[w] = upto;
   __syncthreads();
-  unsigned key[STEPS];
   unsigned long long same[STEPS];                             // lanes with the same digit in each step
-#pragma unroll
-  for (int s = 0; s < STEPS; s++) {
-    const long t = t0 + s * 64 + lane;
-    key[s] = t < n ? (keys_in ? keys_in[t] : emb_key(ids, t, rows)) : 0u;
-  }
 #pragma unroll
   for (int s = 0; s < STEPS; s++) {
     const bool in = t0 + s * 64 + lane < n;
@@ -244,11 +267,12 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I* __restrict_
   int base = upto - sum;
 #pragma unroll
   for (int i = 0; i < 3; i++) base += i < w ? part[i] : 0;
-  for (int i = 0; i < per; i++) {
-    const int d = tid * per + i;
-    if (d < bins) {
-      int p = base + hist[(long)blockIdx.x * bins + d];
-      base += total[d];
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const int d = tid * PER + i;
+    if (d < used) {
+      int p = base + before_tile[i];
+      base += tot[i];
 #pragma unroll
       for (int q = 0; q < 4; q++) {
         const int c = off[q][d];
@@ -270,7 +294,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I* __restrict_
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (in) {
       keys_out[p + before] = key[s];
-      order_out[p + before] = order_in ? order_in[t] : (int)t;
+      order_out[p + before] = from[s];
     }
   }
 }
@@ -293,19 +317,20 @@ __global__ __launch_bounds__(TILE) void embed_pass_kernel(const I* __restrict__ 
   unsigned short* off = reinterpret_cast<unsigned short*>(lds + 2 * ONE_COPIES * bins);    // (places below ONE_MAX)
   for (int i = tid; i < (2 * ONE_COPIES + ONE_WAVES / 2) * bins; i += TILE) lds[i] = 0;
   __syncthreads();
-  unsigned key = 0;
-#pragma unroll 4
-  for (int b = 0; b < n; b += TILE) {
-    const int i = b + tid;
-    if (i < n) {
-      const unsigned k = keys_in ? keys_in[i] : emb_key(ids, i, rows);
-      const int d = (k >> shift) & (bins - 1);
-      atomicAdd(&cnt[((b < t0 ? 0 : bins) + d) * ONE_COPIES + copy], 1);
-      if (b == t0) key = k;
-    }
-  }
   const int t = t0 + tid;
   const bool in = t < n;
+  const unsigned key = emb_key_at(ids, keys_in, min(t, n - 1), rows);
+  const int from = order_in ? order_in[min(t, n - 1)] : t;
+  constexpr int U = 16;                                    // loads in flight
+  for (int b = 0; b < n; b += U * TILE) {
+    unsigned k[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) k[u] = b + u * TILE < n ? emb_key_at(ids, keys_in, min(b + u * TILE + tid, n - 1), rows) : 0u;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (b + u * TILE + tid < n)
+        atomicAdd(&cnt[((b + u * TILE < t0 ? 0 : bins) + ((k[u] >> shift) & (bins - 1))) * ONE_COPIES + copy], 1);
+  }
   const int d = (key >> shift) & (bins - 1);
   const unsigned long long same = emb_same_digit(d, bits, in);
   const int before = __popcll(same & ((1ull << lane) - 1));
@@ -344,7 +369,7 @@ __global__ __launch_bounds__(TILE) void embed_pass_kernel(const I* __restrict__ 
   if (in) {
     const int p = off[w * bins + d] + before;
     keys_out[p] = key;
-    order_out[p] = order_in ? order_in[t] : t;
+    order_out[p] = from;
   }
 }
 
@@ -376,70 +401,52 @@ __device__ __forceinline__ int emb_lower_bound_wave(const unsigned* __restrict__
   return lo;
 }
 
-// grid (shares, then workgroups that write the rows without tokens; pieces of the columns).  A share is what a workgroup sums: `group`
-// places per group of lanes, (256 >> ls) groups.  The groups sum their runs in registers and meet in LDS, so that only the run that
-// enters the share and the one that leaves it become partial rows: part [shares][2][D], row 0 entered, row 1 begins here and leaves.
-template <typename T, typename G>
-__global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ dout, long dstride, const unsigned* __restrict__ keys,
-                                                        const int* __restrict__ order, int n, unsigned rows, int D, int ls, int group,
-                                                        int shares, float scale, G* __restrict__ grad, float* __restrict__ part) {
-  constexpr int V = row_vec<T>();
-  const int tid = threadIdx.x;
-  if ((int)blockIdx.x >= shares) {                           // rows that no token names
-    const int lane = tid & 63;
-    const long r0 = ((long)((int)blockIdx.x - shares) * 4 + (tid >> 6)) * ZERO_ROWS;
-    if (r0 >= (long)rows) return;
-    const int lo = emb_lower_bound_wave(keys, 0, n, (unsigned)r0);
-    const unsigned next = lo + lane < n ? keys[lo + lane] : 0xffffffffu;
-    bool empty = false;
-    if (__ballot(next >= (unsigned)r0 + ZERO_ROWS)) {          // 64 places show all tokens of these rows
-#pragma unroll
-      for (int i = 0; i < ZERO_ROWS; i++) {
-        const bool none = __ballot(next == (unsigned)r0 + i) == 0;
-        if (lane == i) empty = none && r0 + i < (long)rows;
-      }
-    } else if (lane < ZERO_ROWS && r0 + lane < (long)rows) {
-      const unsigned r = (unsigned)(r0 + lane);
-      const int p = emb_lower_bound(keys, lo, n, r);
-      empty = p >= n || keys[p] != r;
-    }
-    unsigned long long m = __ballot(empty);
-    const int c0 = (int)blockIdx.y * (V << ls), c1 = min(D, c0 + (V << ls));
-    constexpr int VG = row_vec<G>();
-    float z[VG];
-#pragma unroll
-    for (int i = 0; i < VG; i++) z[i] = 0.0f;
-    while (m) {
-      const int i = __ffsll(m) - 1;
-      m &= m - 1;
-      G* g = grad + (r0 + i) * (long)D;
-      for (int c = c0 + lane * VG; c < c1; c += 64 * VG) row_store<G, VG, true>(g, c, c1, z);
-    }
-    return;
-  }
+// The sums of one workgroup over its share of a sorted list of n places: groups of 1 << ls lanes take `group` places each from `base` on and
+// sum runs of equal keys in registers; runs that cross groups meet through shuffles and LDS.  key(p), token(p): the list; `from`: dout at
+// the lane's columns.  done(key, sum): a run that lies inside the share; enter(sum), leave(sum): the part of the run that enters the
+// share, of the one that leaves it.
+template <typename T, int V, typename Key, typename Token, typename Done, typename Enter, typename Leave>
+__device__ __forceinline__ void emb_sum_share(const T* __restrict__ from, long dstride, long base, int n, unsigned rows, int ls, int group,
+                                              Key key, Token token, Done done, Enter enter, Leave leave) {
+  const int tid = threadIdx.x, lane = tid & ((1 << ls) - 1);
   __shared__ float met[4][64][V + 1];                        // per wave: the run that was open where its first group begins
   __shared__ bool on[4];                                     // ... and whether it is still open where the wave ends
-  const int lane = tid & ((1 << ls) - 1), gi = tid >> ls, groups = 256 >> ls;
-  const int c = (int)blockIdx.y * (V << ls) + lane * V;
-  const long p0l = ((long)blockIdx.x * groups + gi) * group;
+  const int gi = tid >> ls;
+  const long p0l = base + (long)gi * group;
   const int p0 = (int)min(p0l, (long)n), p1 = min(p0 + group, n);
-  unsigned cur = p0 < p1 ? keys[p0] : rows;
-  bool head = p0 > 0 && p0 < p1 && keys[p0 - 1] == cur;
-  const bool open = p0 < p1 && p1 < n && keys[p1] == keys[p1 - 1];
+  unsigned cur = p0 < p1 ? key(p0) : rows;
+  bool head = p0 > 0 && p0 < p1 && key(p0 - 1) == cur;
+  const bool open = p0 < p1 && p1 < n && key(p1) == key(p1 - 1);
   const bool entered = head && cur < rows;                    // by a run that began before
   bool through = false, leaves = false;                        // that run goes on behind the group; another one does
   float in[V], acc[V];                                         // the sum of that run here; of the current run
 #pragma unroll
   for (int i = 0; i < V; i++) in[i] = acc[i] = 0.0f;
-  constexpr int U = 8;
+  // SUM_U rows on their way at a time, and the next ones' places (padded places' rows are read like others: their sum goes nowhere)
+  constexpr int U = SUM_U;
+  unsigned kn[U];
+  int next[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const int p = max(min(p0 + u, p1 - 1), 0);
+    kn[u] = p0 < p1 ? key(p) : rows;
+    next[u] = p0 < p1 ? token(p) : 0;
+  }
   for (int b = p0; b < p1; b += U) {
     unsigned k[U];
     RowPiece<T, V> v[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int p = min(b + u, p1 - 1);
-      k[u] = keys[p];
-      v[u] = row_load<T, V>(dout + (long)order[p] * dstride, c, k[u] < rows ? D : 0);
+      k[u] = kn[u];
+      v[u] = row_get<T, V>(from + (long)next[u] * dstride);
+    }
+    if (b + U < p1) {
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int p = min(b + U + u, p1 - 1);
+        kn[u] = key(p);
+        next[u] = token(p);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -449,9 +456,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
 #pragma unroll
           for (int i = 0; i < V; i++) in[i] = acc[i];
         } else {
-#pragma unroll
-          for (int i = 0; i < V; i++) acc[i] *= scale;
-          row_store<G, V, true>(grad + (long)cur * D, c, D, acc);
+          done(cur, acc);
         }
         head = false;
         cur = k[u];
@@ -470,9 +475,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
     } else if (open) {
       leaves = true;
     } else {
-#pragma unroll
-      for (int i = 0; i < V; i++) acc[i] *= scale;
-      row_store<G, V, true>(grad + (long)cur * D, c, D, acc);
+      done(cur, acc);
     }
   }
   // what follows in the wave: in = sum of the entering run from this group to its end or the wave's, doubling the reach step by step
@@ -503,12 +506,11 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
     through = last || goes;                                    // (of the leaving run from here on)
   }
   __syncthreads();
-  float* mine = part + (long)blockIdx.x * 2 * D;
   if (gi == 0 && entered) {                                    // the run that enters the share
     for (int j = 1; j < 4 && on[j - 1]; j++)
 #pragma unroll
       for (int i = 0; i < V; i++) in[i] += met[j][wl][i];
-    row_store<float, V>(mine, c, D, in);
+    enter(in);
   }
   if (leaves) {
     for (int j = w + 1; j < 4 && through; j++) {
@@ -517,13 +519,62 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
       through = on[j];
     }
     if (through) {
-      row_store<float, V>(mine + D, c, D, acc);
+      leave(acc);
     } else {
-#pragma unroll
-      for (int i = 0; i < V; i++) acc[i] *= scale;
-      row_store<G, V, true>(grad + (long)cur * D, c, D, acc);
+      done(cur, acc);
     }
   }
+}
+
+// grid: (shares, then workgroups that write the rows without tokens) x pieces of the columns, the pieces of one share next to each
+// other, so that the rows of dout are read whole at about the same time.  A share is what a workgroup sums: `group`
+// places per group of lanes, (256 >> ls) groups.  The groups sum their runs in registers and meet in LDS, so that only the run that
+// enters the share and the one that leaves it become partial rows: part [shares][2][D], row 0 entered, row 1 begins here and leaves.
+template <typename T, int V, typename G>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ dout, long dstride, const unsigned* __restrict__ keys,
+                                                        const int* __restrict__ order, int n, unsigned rows, int D, int ls, int group,
+                                                        int shares, int pieces, float scale, G* __restrict__ grad,
+                                                        float* __restrict__ part) {
+  const int tid = threadIdx.x, block = (int)(blockIdx.x / (unsigned)pieces), lane = tid & ((1 << ls) - 1);
+  const int first = (int)(blockIdx.x - (unsigned)block * pieces) * (V << ls) + lane * V, c = min(first, D - V);
+  const bool col = first < D;
+  if (block >= shares) {                           // rows that no token names
+    const int wl = tid & 63;
+    const long r0 = ((long)(block - shares) * 4 + (tid >> 6)) * ZERO_ROWS;
+    if (r0 >= (long)rows) return;
+    const int lo = emb_lower_bound_wave(keys, 0, n, (unsigned)r0);
+    const unsigned next = lo + wl < n ? keys[lo + wl] : 0xffffffffu;
+    bool empty = false;
+    if (__ballot(next >= (unsigned)r0 + ZERO_ROWS)) {          // 64 places show all tokens of these rows
+#pragma unroll
+      for (int i = 0; i < ZERO_ROWS; i++) {
+        const bool none = __ballot(next == (unsigned)r0 + i) == 0;
+        if (wl == i) empty = none && r0 + i < (long)rows;
+      }
+    } else if (wl < ZERO_ROWS && r0 + wl < (long)rows) {
+      const unsigned r = (unsigned)(r0 + wl);
+      const int p = emb_lower_bound(keys, lo, n, r);
+      empty = p >= n || keys[p] != r;
+    }
+    const unsigned long long m = __ballot(empty);
+    float z[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) z[i] = 0.0f;
+    for (int i = wl >> ls; i < ZERO_ROWS; i += 64 >> ls)
+      if (col && ((m >> i) & 1)) row_put<G, V, true>(grad + (r0 + i) * D + c, z);
+    return;
+  }
+  auto store = [&](unsigned r, float* acc) {
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] *= scale;
+    if (col) row_put<G, V, true>(grad + (long)r * D + c, acc);
+  };
+  auto keep = [&](float* acc, int k) {
+    if (col) row_put<float, V, false>(part + ((long)block * 2 + k) * D + c, acc);
+  };
+  emb_sum_share<T, V>(
+      dout + c, dstride, (long)block * group * (256 >> ls), n, rows, ls, group, [&](int p) { return keys[p]; },
+      [&](int p) { return order[p]; }, store, [&](float* acc) { keep(acc, 0); }, [&](float* acc) { keep(acc, 1); });
 }
 
 // grid (`each` shares each, pieces of the columns): a run that crosses the end of the share in which it begins is finished here.
@@ -534,7 +585,8 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const unsigned* __restr
                                                          int each) {
   __shared__ float red[256][V + 1];
   const int tid = threadIdx.x, sub = tid >> ls, subs = 256 >> ls;
-  const int c = (int)blockIdx.y * (V << ls) + (tid & ((1 << ls) - 1)) * V;
+  const int first = (int)blockIdx.y * (V << ls) + (tid & ((1 << ls) - 1)) * V, c = min(first, D - V);
+  const bool col = first < D;
   bool mine = false;                                           // every wave finds the same shares
   {
     const int i = tid & 63;
@@ -550,15 +602,19 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const unsigned* __restr
     todo &= todo - 1;
     const int p1 = (g + 1) * share;
     const unsigned cur = keys[p1];
-    const int end = emb_lower_bound_wave(keys, p1, n, cur + 1u);
-    const int m = (end - 1) / share - g + 1;                   // partial rows: [g][1], [g + 1][0], [g + 2][0], ...
+    // partial rows: [g][1], [g + 1][0], [g + 2][0], ...: one for every share that the run enters.  64 shares' beginnings are looked at;
+    // a longer run is searched for
+    const long begin = p1 + ((long)(tid & 63) + 1) * share;
+    const unsigned long long enters = __ballot(begin < n && keys[begin < n ? begin : p1] == cur);
+    int m = 2 + __popcll(enters);
+    if (enters == ~0ull) m = (emb_lower_bound_wave(keys, p1, n, cur + 1u) - 1) / share - g + 1;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] = 0.0f;
-    if (c < D) {
+    if (col) {
 #pragma unroll 8
       for (int i = sub; i < m; i += subs) {
-        const RowPiece<float, V> v = row_load<float, V>(part + ((long)(g + i) * 2 + (i == 0 ? 1 : 0)) * D, c, D);
+        const RowPiece<float, V> v = row_get<float, V>(part + ((long)(g + i) * 2 + (i == 0 ? 1 : 0)) * D + c);
 #pragma unroll
         for (int e = 0; e < V; e++) acc[e] += v.e[e];
       }
@@ -567,33 +623,162 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const unsigned* __restr
 #pragma unroll
     for (int e = 0; e < V; e++) red[tid][e] = acc[e];
     __syncthreads();
-    if (sub == 0 && c < D) {
+    if (sub == 0 && col) {
       for (int s = 1; s < min(subs, m); s++)
 #pragma unroll
         for (int e = 0; e < V; e++) acc[e] += red[(s << ls) + tid][e];
 #pragma unroll
       for (int e = 0; e < V; e++) acc[e] *= scale;
-      row_store<G, V, true>(grad + (long)cur * D, c, D, acc);
+      row_put<G, V, true>(grad + (long)cur * D + c, acc);
     }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few, narrow rows and many tokens (the samples of a training step and their keyframes' latents): two launches instead of five.  A
+// workgroup sorts its TILE tokens in LDS and leaves one sum per row that occurs among them, part [rows][tiles][D], and a bit for it in
+// touched [tiles][32]; then a workgroup per row adds the tiles' sums in order.
+// ---------------------------------------------------------------------------------------------
+template <typename T, int V, typename I>
+__global__ __launch_bounds__(256) void embed_tile_kernel(const T* __restrict__ dout, long dstride, const I* __restrict__ ids, int n,
+                                                         unsigned rows, int D, int ls, int tiles, float* __restrict__ part,
+                                                         unsigned* __restrict__ touched) {
+  __shared__ int off[4][MAX_BINS];
+  __shared__ unsigned short key_of[TILE], token_of[TILE];
+  __shared__ unsigned bits[MAX_BINS / 32];
+  __shared__ int sums[4];
+  constexpr int STEPS = TILE / 256, PER = MAX_BINS / 256;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tile = blockIdx.x;
+  const int t0 = tile * TILE, have = min(n - t0, TILE);
+  unsigned key[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; s++) key[s] = emb_key(ids[t0 + min((w * STEPS + s) * 64 + lane, have - 1)], rows);
+  for (int i = tid; i < 4 * MAX_BINS; i += 256) off[i / MAX_BINS][i % MAX_BINS] = 0;
+  if (tid < MAX_BINS / 32) bits[tid] = 0;
+  __syncthreads();
+  unsigned long long same[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; s++) {
+    const bool in = (w * STEPS + s) * 64 + lane < have;
+    same[s] = emb_same_digit((int)key[s], MAX_BITS, in);
+    if (in && (same[s] & ((1ull << lane) - 1)) == 0) off[w][key[s]] += __popcll(same[s]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();
+  int tot[PER], sum = 0;                                       // (thread: PER neighbouring rows)
+  unsigned seen = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    tot[i] = off[0][tid * PER + i] + off[1][tid * PER + i] + off[2][tid * PER + i] + off[3][tid * PER + i];
+    seen |= tot[i] ? 1u << i : 0u;
+    sum += tot[i];
+  }
+  if (seen) atomicOr(&bits[tid * PER / 32], seen << (tid * PER % 32));
+  int upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int from = __shfl_up(upto, o, 64);
+    upto += lane >= o ? from : 0;
+  }
+  if (lane == 63) sums[w] = upto;
+  __syncthreads();
+  int at = upto - sum;
+#pragma unroll
+  for (int i = 0; i < 3; i++) at += i < w ? sums[i] : 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++)
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int c = off[q][tid * PER + i];
+      off[q][tid * PER + i] = at;
+      at += c;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < STEPS; s++) {
+    const int t = (w * STEPS + s) * 64 + lane;
+    const bool in = t < have;
+    const int before = __popcll(same[s] & ((1ull << lane) - 1));
+    const int p = in ? off[w][key[s]] : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in && before == 0) off[w][key[s]] = p + __popcll(same[s]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in) {
+      key_of[p + before] = (unsigned short)key[s];
+      token_of[p + before] = (unsigned short)t;
+    }
+  }
+  __syncthreads();
+  if (tid < MAX_BINS / 32) touched[(long)tile * (MAX_BINS / 32) + tid] = bits[tid];
+  const int first = (tid & ((1 << ls) - 1)) * V, c = min(first, D - V);
+  const bool col = first < D;
+  auto store = [&](unsigned r, float* acc) {
+    if (col) row_put<float, V, false>(part + ((long)r * tiles + tile) * D + c, acc);
+  };
+  // (nothing enters or leaves: the share is the whole list)
+  emb_sum_share<T, V>(
+      dout + (long)t0 * dstride + c, dstride, 0, have, rows, ls, (TILE / 256) << ls, [&](int p) { return (unsigned)key_of[p]; },
+      [&](int p) { return (int)token_of[p]; }, store, [](float*) {}, [](float*) {});
+}
+
+// one workgroup per row
+template <typename G, int V>
+__global__ __launch_bounds__(256) void embed_rows_kernel(const float* __restrict__ part, const unsigned* __restrict__ touched, int tiles,
+                                                         int D, int ls, float scale, G* __restrict__ grad) {
+  __shared__ float red[256][V + 1];
+  const int tid = threadIdx.x, sub = tid >> ls, subs = 256 >> ls;
+  const int row = blockIdx.x;
+  const int first = (tid & ((1 << ls) - 1)) * V, c = min(first, D - V);
+  const float* from = part + (long)row * tiles * D + c;
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) acc[i] = 0.0f;
+  constexpr int U = 8;
+  for (int t = sub; t < tiles; t += U * subs) {
+    unsigned word[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) word[u] = t + u * subs < tiles ? touched[(long)(t + u * subs) * (MAX_BINS / 32) + (row >> 5)] : 0u;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if ((word[u] >> (row & 31)) & 1) {
+        const RowPiece<float, V> v = row_get<float, V>(from + (long)(t + u * subs) * D);
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] += v.e[i];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) red[tid][i] = acc[i];
+  for (int o = subs / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (sub < o) {
+#pragma unroll
+      for (int i = 0; i < V; i++) red[tid][i] += red[tid + (o << ls)][i];
+    }
+  }
+  if (sub == 0 && first < D) {
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] = red[tid][i] * scale;
+    row_put<G, V, true>(grad + (long)row * D + c, acc);
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // C ABI
 // ---------------------------------------------------------------------------------------------
-// limits that keep every grid below 2^32 threads (a group of up to 64 lanes per 16 tokens, 4 lanes per table row) and places in 32 bits
+// limits that keep every grid below 2^32 threads (up to 64 lanes per token, 8 per table row) and places in 32 bits
 #define EMB_MAX_COLS 65536
-#define EMB_MAX_TOKENS (1L << 27)
+#define EMB_MAX_TOKENS (1L << 25)
 #define EMB_MAX_ROWS (1L << 29)
 
 struct EmbPlan {
-  bool ranked;
+  bool ranked, few;
   int passes, bits, tiles, ls, group, shares;
-  size_t keys[2], order[2], hist, total, part, bytes;
+  size_t keys[2], order[2], hist, total, part, touched, bytes;
 };
 
 static EmbPlan emb_plan(long n, long rows, int cols, int vec) {
-  EmbPlan p;
+  EmbPlan p = {};
   p.ranked = n <= RANK_MAX;
   int need = 1;
   while (need < 32 && ((unsigned long)rows >> need) != 0) need++;         // keys 0 .. rows
@@ -612,6 +797,13 @@ static EmbPlan emb_plan(long n, long rows, int cols, int vec) {
     at += (b + 255) & ~(size_t)255;
     return was;
   };
+  p.few = !p.ranked && rows <= FEW_ROWS && p.ls <= FEW_LANES && p.tiles <= FEW_TILES;
+  if (p.few) {
+    p.touched = take((size_t)p.tiles * (MAX_BINS / 8));
+    p.part = take((size_t)rows * p.tiles * cols * 4);
+    p.bytes = at;
+    return p;
+  }
   for (int i = 0; i < 2; i++) {
     p.keys[i] = take(i == 0 || p.passes > 1 ? 4 * (size_t)n : 0);
     p.order[i] = take(i == 0 || p.passes > 1 ? 4 * (size_t)n : 0);
@@ -623,13 +815,29 @@ static EmbPlan emb_plan(long n, long rows, int cols, int vec) {
   return p;
 }
 
+template <int N>
+struct EmbInt { static constexpr int v = N; };
+
+// calls f(V): the elements that a lane holds of a row of D
+template <typename T, typename F>
+static void emb_pieces(int D, F f) {
+  if (D >= row_vec<T>()) f(EmbInt<row_vec<T>()>());
+  else f(EmbInt<1>());
+}
+
+// the same number, for a dtype of the C ABI
+static int emb_vec(int dtype, int D) {
+  const int v = dtype == NS_F32 ? 4 : 8;
+  return D >= v ? v : 1;
+}
+
 static inline bool emb_type(int dtype) { return dtype == NS_F16 || dtype == NS_BF16 || dtype == NS_F32; }
 
-template <typename T, typename I>
+template <typename T, int V, typename I>
 static void emb_forward(const void* table, long tstride, const void* ids, void* out, long n, long rows, int cols, float scale,
                         hipStream_t s) {
-  const int ls = row_lanes_log2(cols, row_vec<T>());
-  hipLaunchKernelGGL((embed_fwd_kernel<T, I>), dim3((unsigned)((n + (256 >> ls) * EMB_U - 1) / ((256 >> ls) * EMB_U))), dim3(256), 0, s,
+  const int ls = row_lanes_log2(cols, V);
+  hipLaunchKernelGGL((embed_fwd_kernel<T, V, I>), dim3((unsigned)((n + (256 >> ls) - 1) / (256 >> ls))), dim3(256), 0, s,
                      (const T*)table, tstride, (const I*)ids, (T*)out, n, (unsigned)rows, cols, ls, scale);
 }
 
@@ -640,12 +848,15 @@ extern "C" int ns_embedding_forward(const void* table, long table_stride, const 
   if (n == 0) return NS_OK;
   NS_REQUIRE(ids && out && (table || rows == 0), "ns_embedding_forward: null pointer");
   NS_REQUIRE(n <= EMB_MAX_TOKENS && rows <= EMB_MAX_ROWS && cols >= 1 && cols <= EMB_MAX_COLS && table_stride >= 0,
-             "ns_embedding_forward: bad shape (n %ld <= 2^27, rows %ld <= 2^29, cols %d in 1 .. %d)", n, rows, cols, EMB_MAX_COLS);
+             "ns_embedding_forward: bad shape (n %ld <= 2^25, rows %ld <= 2^29, cols %d in 1 .. %d)", n, rows, cols, EMB_MAX_COLS);
   hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (ids_are_64) emb_forward<T, int64_t>(table, table_stride, ids, out, n, rows, cols, scale, s);
-    else emb_forward<T, int32_t>(table, table_stride, ids, out, n, rows, cols, scale, s);
+    emb_pieces<T>(cols, [&](auto piece) {
+      constexpr int V = decltype(piece)::v;
+      if (ids_are_64) emb_forward<T, V, int64_t>(table, table_stride, ids, out, n, rows, cols, scale, s);
+      else emb_forward<T, V, int32_t>(table, table_stride, ids, out, n, rows, cols, scale, s);
+    });
   };
   if (dtype == NS_F16) go((_Float16)0);
   else if (dtype == NS_BF16) go((rw_bf16)0.0f);
@@ -656,7 +867,7 @@ extern "C" int ns_embedding_forward(const void* table, long table_stride, const 
 
 extern "C" size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols, int dtype) {
   if (n <= 0 || n > EMB_MAX_TOKENS || rows < 0 || rows > EMB_MAX_ROWS || cols < 1 || cols > EMB_MAX_COLS) return 0;
-  return emb_plan(n, rows, cols, dtype == NS_F32 ? 4 : 8).bytes;
+  return emb_plan(n, rows, cols, emb_vec(dtype, cols)).bytes;
 }
 
 template <typename I>
@@ -665,7 +876,7 @@ static void emb_sort(const EmbPlan& p, const I* ids, char* ws, int n, unsigned r
   unsigned* k[2] = {(unsigned*)(ws + p.keys[0]), (unsigned*)(ws + p.keys[1])};
   int* o[2] = {(int*)(ws + p.order[0]), (int*)(ws + p.order[1])};
   if (p.ranked) {
-    hipLaunchKernelGGL(embed_rank_kernel<I>, dim3((n + 63) / 64), dim3(64 * RANK_WAVES), 0, s, ids, n, rows, k[0], o[0]);
+    hipLaunchKernelGGL(embed_rank_kernel<I>, dim3((n + RANK_TOKENS - 1) / RANK_TOKENS), dim3(64 * RANK_WAVES), 0, s, ids, n, rows, k[0], o[0]);
     *keys = k[0];
     *order = o[0];
     return;
@@ -683,10 +894,11 @@ static void emb_sort(const EmbPlan& p, const I* ids, char* ws, int n, unsigned r
       oi = o[i & 1];
       continue;
     }
-    hipLaunchKernelGGL(embed_hist_kernel<I>, dim3(p.tiles), dim3(256), 0, s, ids, ki, (long)n, rows, i * p.bits, bins, hist);
-    hipLaunchKernelGGL(embed_prefix_kernel, dim3((bins + 63) / 64), dim3(1024), 0, s, hist, p.tiles, bins, total);
-    hipLaunchKernelGGL(embed_scatter_kernel<I>, dim3(p.tiles), dim3(256), 0, s, ids, ki, oi, (long)n, rows, i * p.bits, p.bits, hist,
-                       total, k[i & 1], o[i & 1]);
+    const int used = (int)min((unsigned)bins, (rows >> (i * p.bits)) + 1);      // digits that occur: the keys end at `rows`
+    hipLaunchKernelGGL(embed_hist_kernel<I>, dim3(p.tiles), dim3(256), 0, s, ids, ki, (long)n, rows, i * p.bits, bins, used, hist);
+    hipLaunchKernelGGL(embed_prefix_kernel, dim3((used + 63) / 64), dim3(1024), 0, s, hist, p.tiles, used, total);
+    hipLaunchKernelGGL(embed_scatter_kernel<I>, dim3(p.tiles), dim3(256), 0, s, ids, ki, oi, (long)n, rows, i * p.bits, p.bits, used,
+                       hist, total, k[i & 1], o[i & 1]);
     ki = k[i & 1];
     oi = o[i & 1];
   }
@@ -694,14 +906,23 @@ static void emb_sort(const EmbPlan& p, const I* ids, char* ws, int n, unsigned r
   *order = oi;
 }
 
-template <typename T, typename G>
+template <typename T, int V, typename G, typename I>
+static void emb_few(const EmbPlan& p, const T* dout, long dstride, const I* ids, int n, unsigned rows, int cols, float scale, G* grad,
+                    char* ws, hipStream_t s) {
+  float* part = (float*)(ws + p.part);
+  unsigned* touched = (unsigned*)(ws + p.touched);
+  hipLaunchKernelGGL((embed_tile_kernel<T, V, I>), dim3(p.tiles), dim3(256), 0, s, dout, dstride, ids, n, rows, cols, p.ls, p.tiles, part,
+                     touched);
+  hipLaunchKernelGGL((embed_rows_kernel<G, V>), dim3(rows), dim3(256), 0, s, part, touched, p.tiles, cols, p.ls, scale, grad);
+}
+
+template <typename T, int V, typename G>
 static void emb_sums(const EmbPlan& p, const T* dout, long dstride, const unsigned* keys, const int* order, int n, unsigned rows,
                      int cols, float scale, G* grad, float* part, hipStream_t s) {
-  constexpr int V = row_vec<T>();
   const int zero_blocks = (int)(((long)rows + 4 * ZERO_ROWS - 1) / (4 * ZERO_ROWS));
   const int col_blocks = (cols + (V << p.ls) - 1) / (V << p.ls), share = p.group * (256 >> p.ls);
-  hipLaunchKernelGGL((embed_sum_kernel<T, G>), dim3(p.shares + zero_blocks, col_blocks), dim3(256), 0, s, dout, dstride, keys, order, n,
-                     rows, cols, p.ls, p.group, p.shares, scale, grad, part);
+  hipLaunchKernelGGL((embed_sum_kernel<T, V, G>), dim3((unsigned)(p.shares + zero_blocks) * col_blocks), dim3(256), 0, s, dout, dstride, keys,
+                     order, n, rows, cols, p.ls, p.group, p.shares, col_blocks, scale, grad, part);
   if (p.shares > 1) {
     // one workgroup per share up to 1024 of them (in a skewed list most are the beginning of a crossing run, each a chain of loads);
     // beyond, a workgroup looks at up to 64
@@ -720,14 +941,14 @@ extern "C" int ns_embedding_backward(const void* dout, long dout_stride, int dty
   if (rows == 0) return NS_OK;
   NS_REQUIRE(grad && (n == 0 || (dout && ids && ws)), "ns_embedding_backward: null pointer");
   NS_REQUIRE(n <= EMB_MAX_TOKENS && rows <= EMB_MAX_ROWS && cols >= 1 && cols <= EMB_MAX_COLS && dout_stride >= 0,
-             "ns_embedding_backward: bad shape (n %ld <= 2^27, rows %ld <= 2^29, cols %d in 1 .. %d)", n, rows, cols, EMB_MAX_COLS);
-  const EmbPlan p = emb_plan(n, rows, cols, dtype == NS_F32 ? 4 : 8);
+             "ns_embedding_backward: bad shape (n %ld <= 2^25, rows %ld <= 2^29, cols %d in 1 .. %d)", n, rows, cols, EMB_MAX_COLS);
+  const EmbPlan p = emb_plan(n, rows, cols, emb_vec(dtype, cols));
   NS_REQUIRE(n == 0 || ws_bytes >= p.bytes, "ns_embedding_backward: workspace of %zu bytes, %zu needed", ws_bytes, p.bytes);
   NS_REQUIRE(((uintptr_t)ws % 16) == 0, "ns_embedding_backward: the workspace needs 16-byte alignment");
   hipStream_t s = (hipStream_t)stream;
   const unsigned* keys = nullptr;
   const int* order = nullptr;
-  if (n > 0) {
+  if (n > 0 && !p.few) {
     if (ids_are_64) emb_sort(p, (const int64_t*)ids, (char*)ws, (int)n, (unsigned)rows, &keys, &order, s);
     else emb_sort(p, (const int32_t*)ids, (char*)ws, (int)n, (unsigned)rows, &keys, &order, s);
     NS_CHECK_LAUNCH("embedding_backward: sort");
@@ -735,10 +956,21 @@ extern "C" int ns_embedding_backward(const void* dout, long dout_stride, int dty
   auto go = [&](auto t) {
     using T = decltype(t);
     float* part = (float*)((char*)ws + p.part);
-    if (grad_dtype == NS_F32)
-      emb_sums<T, float>(p, (const T*)dout, dout_stride, keys, order, (int)n, (unsigned)rows, cols, scale, (float*)grad, part, s);
-    else
-      emb_sums<T, T>(p, (const T*)dout, dout_stride, keys, order, (int)n, (unsigned)rows, cols, scale, (T*)grad, part, s);
+    emb_pieces<T>(cols, [&](auto piece) {
+      constexpr int V = decltype(piece)::v;
+      auto few = [&](auto* g) {
+        if (ids_are_64) emb_few<T, V>(p, (const T*)dout, dout_stride, (const int64_t*)ids, (int)n, (unsigned)rows, cols, scale, g, (char*)ws, s);
+        else emb_few<T, V>(p, (const T*)dout, dout_stride, (const int32_t*)ids, (int)n, (unsigned)rows, cols, scale, g, (char*)ws, s);
+      };
+      if (p.few && grad_dtype == NS_F32)
+        few((float*)grad);
+      else if (p.few)
+        few((T*)grad);
+      else if (grad_dtype == NS_F32)
+        emb_sums<T, V, float>(p, (const T*)dout, dout_stride, keys, order, (int)n, (unsigned)rows, cols, scale, (float*)grad, part, s);
+      else
+        emb_sums<T, V, T>(p, (const T*)dout, dout_stride, keys, order, (int)n, (unsigned)rows, cols, scale, (T*)grad, part, s);
+    });
   };
   if (dtype == NS_F16) go((_Float16)0);
   else if (dtype == NS_BF16) go((rw_bf16)0.0f);

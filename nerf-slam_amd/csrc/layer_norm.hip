@@ -46,11 +46,6 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2]) {
   }
 }
 
-#ifdef LN512
-#define LNX LnInt<512>(), LnInt<2>()
-#else
-#define LNX LnInt<256>(), LnInt<4>()
-#endif
 template <int LPR>
 constexpr int ln_block() { return LPR > 256 ? LPR : 256; }
 
@@ -140,10 +135,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
     for (int i = 0; i < V; i++) dw[j][i] = db[j][i] = 0.0f;
   }
   // the next row is on its way while this one is worked on, where the registers allow it
-  #ifndef LNAHEAD
-#define LNAHEAD (LPR < 1024 && NV < 4)
-#endif
-  constexpr bool AHEAD = LNAHEAD;
+    constexpr bool AHEAD = LPR < 1024;
   RowPiece<T, V> pn[NV], dn[NV];
   float mun = 0.0f, rsn = 0.0f;
   auto fetch = [&](long r) {
@@ -243,11 +235,13 @@ __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __r
 // C ABI
 // ---------------------------------------------------------------------------------------------
 // Calls f(LPR, NV) with the lanes per row and pieces per lane of a row of D elements.  Up to 128 pieces a wave (or less) holds a row
-// and no barrier is needed; beyond, four waves; beyond 1024 pieces, sixteen.
+// and no barrier is needed; beyond, four waves; beyond 1024 pieces, sixteen.  Of the shapes for 513 .. 1024 pieces the forward pass takes
+// four waves with four pieces per lane, the backward pass, whose sums need the registers, eight waves with two
+// (8192 x 8192 bf16: forward 51 against 56 us, backward 132 against 88).
 template <int N>
 struct LnInt { static constexpr int v = N; };
 
-template <int V, typename F>
+template <int V, bool BACK, typename F>
 static void ln_shape(int D, F f) {
   const int pieces = (D + V - 1) / V;
   if (pieces <= 8) f(LnInt<8>(), LnInt<1>());
@@ -257,7 +251,7 @@ static void ln_shape(int D, F f) {
   else if (pieces <= 128) f(LnInt<64>(), LnInt<2>());
   else if (pieces <= 256) f(LnInt<256>(), LnInt<1>());
   else if (pieces <= 512) f(LnInt<256>(), LnInt<2>());
-  else if (pieces <= 1024) f(LNX);
+  else if (pieces <= 1024) f(LnInt<(BACK ? 512 : 256)>(), LnInt<(BACK ? 2 : 4)>());
   else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
   else if constexpr (V == 4) f(LnInt<1024>(), LnInt<4>());
 }
@@ -274,20 +268,26 @@ static bool ln_types(int dtype, int wdtype, F f) {
   return true;
 }
 
-static int ln_rows_per_block(int D, int vec) {
+// workgroups: enough to fill the chip, few enough that the weights' registers are filled, and (backward) a partial row pair left, once
+// per many rows
+#ifndef LN_F256
+#define LN_F64 8192
+#define LN_F256 4096
+#define LN_F2564 1024
+#define LN_F1024 256
+#endif
+#ifndef LN_B256
+#define LN_B64 768
+#define LN_B256 1024
+#define LN_B2562 512
+#define LN_B512 256
+#define LN_B1024 256
+#endif
+static int ln_blocks(long n, int D, int vec, bool back) {
   const int pieces = (D + vec - 1) / vec;
-  return pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 128 ? 4 : 1;
-}
-
-#ifndef LN_FWD_BLOCKS
-#define LN_FWD_BLOCKS 4096
-#endif
-#ifndef LN_BWD_BLOCKS
-#define LN_BWD_BLOCKS 512
-#endif
-
-static int ln_blocks(long n, int D, int dtype, int most) {
-  const int per = ln_rows_per_block(D, dtype == NS_F32 ? 4 : 8);
+  const int per = pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 128 ? 4 : 1;
+  const int most = pieces <= 128 ? (back ? LN_B64 : LN_F64) : pieces <= 256 ? (back ? LN_B256 : LN_F256)
+                   : pieces <= 512 ? (back ? LN_B2562 : LN_F256) : pieces <= 1024 ? (back ? LN_B512 : LN_F2564) : (back ? LN_B1024 : LN_F1024);
   const long want = (n + per - 1) / per;
   return (int)(want < most ? want : most);
 }
@@ -303,9 +303,9 @@ extern "C" int ns_layer_norm_forward(const void* x, long x_stride, const void* w
   const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
-    ln_shape<row_vec<T>()>(cols, [&](auto lpr, auto nv) {
+    ln_shape<row_vec<T>(), false>(cols, [&](auto lpr, auto nv) {
       constexpr int L = decltype(lpr)::v, N = decltype(nv)::v;
-      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, L, N>), dim3(ln_blocks(n, cols, dtype, LN_FWD_BLOCKS)), dim3(ln_block<L>()), 0,
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, L, N>), dim3(ln_blocks(n, cols, row_vec<T>(), false)), dim3(ln_block<L>()), 0,
                          (hipStream_t)stream, (const T*)x, x_stride, (const W*)weight, (const W*)bias, (T*)y, mean, rstd, n, cols,
                          1.0f / (float)cols, eps);
     });
@@ -317,7 +317,7 @@ extern "C" int ns_layer_norm_forward(const void* x, long x_stride, const void* w
 
 extern "C" size_t ns_layer_norm_backward_workspace_bytes(long n, int cols, int dtype) {
   if (n <= 0 || cols < 1 || cols > LN_MAX_COLS) return 0;
-  return (size_t)ln_blocks(n, cols, dtype, LN_BWD_BLOCKS) * 2 * cols * 4;
+  return (size_t)ln_blocks(n, cols, dtype == NS_F32 ? 4 : 8, true) * 2 * cols * 4;
 }
 
 extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void* x, long x_stride, const float* mean, const float* rstd,
@@ -330,12 +330,12 @@ extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void
              "ns_layer_norm_backward: weight, dweight and dbias come together");
   const size_t need = weight ? ns_layer_norm_backward_workspace_bytes(n, cols, dtype) : 0;
   NS_REQUIRE(ws_bytes >= need && (ws || need == 0), "ns_layer_norm_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  const int blocks = ln_blocks(n, cols, dtype, LN_BWD_BLOCKS);
+  const int blocks = ln_blocks(n, cols, dtype == NS_F32 ? 4 : 8, true);
   const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
     if (n > 0)
-      ln_shape<row_vec<T>()>(cols, [&](auto lpr, auto nv) {
+      ln_shape<row_vec<T>(), true>(cols, [&](auto lpr, auto nv) {
         constexpr int L = decltype(lpr)::v, N = decltype(nv)::v;
         hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, L, N>), dim3(blocks), dim3(ln_block<L>()), 0, (hipStream_t)stream, (const T*)dy,
                            dy_stride, (const T*)x, x_stride, mean, rstd, (const W*)weight, (T*)dx, weight ? (float*)ws : nullptr, n, cols,

@@ -28,29 +28,44 @@ __device__ __forceinline__ RowPiece<T, N> row_load(const T* __restrict__ row, in
   return v;
 }
 
-// STREAM: stores that are not kept in the caches, for outputs that nothing reads while the kernel runs
-template <typename T, int N, bool STREAM = false>
+template <typename T, int N>
 __device__ __forceinline__ void row_store(T* __restrict__ row, int c, int D, const float* f) {
-  typedef int v4i __attribute__((ext_vector_type(4), aligned(2)));     // (an element may be 2 bytes)
   RowPiece<T, N> v;
 #pragma unroll
   for (int i = 0; i < N; i++) v.e[i] = (T)f[i];      // one rounding, to nearest even
   if (c + N <= D) {
-    if (STREAM) {
-      static_assert(!STREAM || sizeof(v) % 16 == 0, "whole 16-byte pieces");
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(v) / 16; i++) {
-        v4i q;
-        __builtin_memcpy(&q, (const char*)&v + 16 * i, 16);
-        __builtin_nontemporal_store(q, reinterpret_cast<v4i*>(row + c) + i);
-      }
-    } else {
-      __builtin_memcpy(row + c, &v, sizeof(v));
-    }
+    __builtin_memcpy(row + c, &v, sizeof(v));
   } else {
 #pragma unroll
     for (int i = 0; i < N; i++)
       if (c + i < D) row[c + i] = v.e[i];
+  }
+}
+
+// whole pieces
+template <typename T, int N>
+__device__ __forceinline__ RowPiece<T, N> row_get(const T* __restrict__ at) {
+  RowPiece<T, N> v;
+  __builtin_memcpy(&v, at, sizeof(v));
+  return v;
+}
+
+// STREAM: stores that are not kept in the caches, for outputs that nothing reads while the kernel runs
+template <typename T, int N, bool STREAM>
+__device__ __forceinline__ void row_put(T* __restrict__ at, const float* f) {
+  typedef int v4i __attribute__((ext_vector_type(4), aligned(2)));     // (an element may be 2 bytes)
+  RowPiece<T, N> v;
+#pragma unroll
+  for (int i = 0; i < N; i++) v.e[i] = (T)f[i];
+  if constexpr (STREAM && sizeof(v) % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(v) / 16; i++) {
+      v4i q;
+      __builtin_memcpy(&q, (const char*)&v + 16 * i, 16);
+      __builtin_nontemporal_store(q, reinterpret_cast<v4i*>(at) + i);
+    }
+  } else {
+    __builtin_memcpy(at, &v, sizeof(v));
   }
 }
 

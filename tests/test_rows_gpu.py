@@ -123,7 +123,8 @@ def check_grad(got, dout, ids, v, scale, what):
 
 
 SIZES = [(1, 1, 1), (1, 40, 16), (15, 3, 5), (16, 3, 8), (17, 3, 8), (33, 1000, 33), (64, 7, 771), (300, 2, 1030), (1000, 64, 32),
-         (8192, 300, 8), (8193, 300, 8), (8193, 1023, 4), (9000, 1024, 12), (20000, 70000, 3), (40000, 5, 16), (4097, 5000, 2050)]
+         (8192, 300, 8), (8193, 300, 8), (8193, 1023, 4), (9000, 1024, 12), (20000, 70000, 3), (40000, 5, 16), (4097, 5000, 2050),
+         (8200, 512, 33), (9300, 512, 64), (30000, 64, 3), (12345, 1, 31), (10240, 513, 32), (9100, 1023, 20), (9200, 1024, 20)]
 
 
 @pytest.mark.parametrize("kind", ["even", "skew", "pad"])
@@ -139,7 +140,7 @@ def test_embedding_backward(dev, n, v, d, kind):
 
 @pytest.mark.parametrize("n,v,d,kind", [
     (300000, 1, 8, "one"), (70000, 9, 40, "one"), (262144, 512, 32, "sorted"), (100000, 1 << 21, 2, "even"), (8192, 10, 16, "none"),
-    (20000, 10, 16, "none"), (5, 1 << 20, 4, "even"), (270000, 3000, 1, "skew"), (12000, 2000, 515, "sorted")])
+    (20000, 10, 16, "none"), (1 << 20, 512, 16, "even"), ((1 << 20) + 5, 512, 8, "skew"), (100000, 300, 60, "one"), (5, 1 << 20, 4, "even"), (270000, 3000, 1, "skew"), (12000, 2000, 515, "sorted")])
 def test_embedding_backward_extremes(dev, n, v, d, kind):
     """one row that takes everything (its partial rows are joined by one workgroup), rows in the millions, three radix passes' worth
     of keys, nothing but padded places, lists beyond one tile of the sort"""

@@ -70,7 +70,7 @@ def test_abi_refusals():
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 7, L(3), L(5), 4, C.c_float(1), None), "dtype")
     _refused(f.ns_embedding_forward(P, L(-1), P, 0, P, 1, L(3), L(5), 4, C.c_float(1), None), "bad shape")
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(-3), L(5), 4, C.c_float(1), None), "bad shape")
-    _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L((1 << 27) + 1), L(5), 4, C.c_float(1), None), "2^27")
+    _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L((1 << 25) + 1), L(5), 4, C.c_float(1), None), "2^25")
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(3), L((1 << 29) + 1), 4, C.c_float(1), None), "2^29")
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(3), L(5), 0, C.c_float(1), None), "bad shape")
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(3), L(5), 65537, C.c_float(1), None), "65536")
@@ -83,7 +83,7 @@ def test_abi_refusals():
     _refused(f.ns_embedding_backward(P, L(4), 2, P, 0, P, 1, L(3), L(5), 4, C.c_float(1), P, big, None), "grad dtype")
     _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(3), L(5), 4, C.c_float(1), P, z, None), "workspace")
     _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(3), L(5), 4, C.c_float(1), C.c_void_p(4100), big, None), "alignment")
-    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L((1 << 27) + 1), L(5), 4, C.c_float(1), P, big, None), "2^27")
+    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L((1 << 25) + 1), L(5), 4, C.c_float(1), P, big, None), "2^25")
     assert f.ns_embedding_backward(None, L(4), 1, None, 0, None, 1, L(3), L(0), 4, C.c_float(1), None, z, None) == 0
 
     e = C.c_float(1e-5)
@@ -110,5 +110,5 @@ def test_workspace_sizes():
     assert emb(L(0), L(5), 4, 1) == 0 and ln(L(0), 4, 2) == 0
     for n in (1, 17, 8192, 8193, 1 << 20):
         assert emb(L(n), L(1000), 64, 2) >= 8 * n and emb(L(n), L(1000), 64, 3) % 16 == 0
-    assert emb(L(1 << 27), L(1 << 29), 8, 1) > 2 ** 31          # (no 32-bit arithmetic in it)
+    assert emb(L(1 << 25), L(1 << 29), 65536, 1) > 2 ** 31          # (no 32-bit arithmetic in it)
     assert ln(L(10), 64, 2) % 512 == 0 and ln(L(1 << 20), 64, 2) > 0
