@@ -747,12 +747,12 @@ int ns_ngp_grid_update_sampled(const void* net_out, const int* cells, int n, flo
  * ---------------------------------------------------------------------------------------- */
 
 /* out[t] = scale * table[ids[t]]; an id outside [0, rows) (a padded place) gives a row of zeros.
- *   table [rows, cols] dtype, ids [n] int32 (int64 if ids_are_64), out [n, cols] dtype; n <= 2^25, rows <= 2^29, cols <= 65536. */
+ *   table [rows, cols] dtype, ids [n] int32 (int64 if ids_are_64), out [n, cols] dtype; n <= 2^25, rows < 2^31, cols <= 65536. */
 int ns_embedding_forward(const void* table, long table_stride, const void* ids, int ids_are_64, void* out, int dtype, long n, long rows,
                          int cols, float scale, void* stream);
 /* grad[r] = scale * sum of dout[t] over the tokens t with ids[t] == r; every row of grad [rows, cols] is written (0 without tokens),
  * rows of dout whose id lies outside [0, rows) are not used.  grad_dtype: dtype or NS_F32.  The tokens are sorted by id on the device
- * and the sums run over the sorted list in a fixed order: the same inputs give the same bits.
+ * and the sums run over the sorted list in a fixed order: the same inputs give the same bits.  rows * ceil(cols / 256) <= 2^27.
  *   ws: ns_embedding_backward_workspace_bytes(n, rows, cols, dtype) bytes, 16-byte aligned, contents irrelevant; calls that may be in flight
  *   at the same time must not share it.                                                                                        */
 size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols, int dtype);

@@ -43,6 +43,16 @@
 #define FEW_LANES 3
 #endif
 #define FEW_TILES 1024
+#ifndef SMALL_MAX
+#define SMALL_MAX 4096       // tokens up to which the gradient is one launch
+#endif
+#define SMALL_ROWS 256       // ... and most rows of the table per workgroup there
+#ifndef SMALL_BLOCKS
+#define SMALL_BLOCKS 256     // workgroups that this form aims at, a quarter of what it takes at most
+#endif
+#ifndef SMALL_LANES
+#define SMALL_LANES 4
+#endif
 
 template <typename I>
 __device__ __forceinline__ unsigned emb_key(I id, unsigned rows) {
@@ -405,12 +415,12 @@ __device__ __forceinline__ int emb_lower_bound_wave(const unsigned* __restrict__
 // sum runs of equal keys in registers; runs that cross groups meet through shuffles and LDS.  key(p), token(p): the list; `from`: dout at
 // the lane's columns.  done(key, sum): a run that lies inside the share; enter(sum), leave(sum): the part of the run that enters the
 // share, of the one that leaves it.
-template <typename T, int V, typename Key, typename Token, typename Done, typename Enter, typename Leave>
+template <typename T, int V, int WAVES, typename Key, typename Token, typename Done, typename Enter, typename Leave>
 __device__ __forceinline__ void emb_sum_share(const T* __restrict__ from, long dstride, long base, int n, unsigned rows, int ls, int group,
                                               Key key, Token token, Done done, Enter enter, Leave leave) {
   const int tid = threadIdx.x, lane = tid & ((1 << ls) - 1);
-  __shared__ float met[4][64][V + 1];                        // per wave: the run that was open where its first group begins
-  __shared__ bool on[4];                                     // ... and whether it is still open where the wave ends
+  __shared__ float met[WAVES][64][V + 1];                        // per wave: the run that was open where its first group begins
+  __shared__ bool on[WAVES];                                   // ... and whether it is still open where the wave ends
   const int gi = tid >> ls;
   const long p0l = base + (long)gi * group;
   const int p0 = (int)min(p0l, (long)n), p1 = min(p0 + group, n);
@@ -507,13 +517,13 @@ __device__ __forceinline__ void emb_sum_share(const T* __restrict__ from, long d
   }
   __syncthreads();
   if (gi == 0 && entered) {                                    // the run that enters the share
-    for (int j = 1; j < 4 && on[j - 1]; j++)
+    for (int j = 1; j < WAVES && on[j - 1]; j++)
 #pragma unroll
       for (int i = 0; i < V; i++) in[i] += met[j][wl][i];
     enter(in);
   }
   if (leaves) {
-    for (int j = w + 1; j < 4 && through; j++) {
+    for (int j = w + 1; j < WAVES && through; j++) {
 #pragma unroll
       for (int i = 0; i < V; i++) acc[i] += met[j][lane][i];
       through = on[j];
@@ -572,7 +582,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
   auto keep = [&](float* acc, int k) {
     if (col) row_put<float, V, false>(part + ((long)block * 2 + k) * D + c, acc);
   };
-  emb_sum_share<T, V>(
+  emb_sum_share<T, V, 4>(
       dout + c, dstride, (long)block * group * (256 >> ls), n, rows, ls, group, [&](int p) { return keys[p]; },
       [&](int p) { return order[p]; }, store, [&](float* acc) { keep(acc, 0); }, [&](float* acc) { keep(acc, 1); });
 }
@@ -717,7 +727,7 @@ __global__ __launch_bounds__(256) void embed_tile_kernel(const T* __restrict__ d
     if (col) row_put<float, V, false>(part + ((long)r * tiles + tile) * D + c, acc);
   };
   // (nothing enters or leaves: the share is the whole list)
-  emb_sum_share<T, V>(
+  emb_sum_share<T, V, 4>(
       dout + (long)t0 * dstride + c, dstride, 0, have, rows, ls, (TILE / 256) << ls, [&](int p) { return (unsigned)key_of[p]; },
       [&](int p) { return (int)token_of[p]; }, store, [](float*) {}, [](float*) {});
 }
@@ -764,28 +774,147 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const float* __restrict
 }
 
 // ---------------------------------------------------------------------------------------------
+// Short lists: everything in one launch.  A workgroup owns `own` neighbouring rows of the table: it picks their tokens out of the whole list,
+// sorts them in LDS, sums them and writes its rows, those without tokens too.  No workspace.
+// grid: groups of rows x pieces of the columns
+// ---------------------------------------------------------------------------------------------
+#define SMALL_STEPS (SMALL_MAX / 1024)
+template <typename T, int V, typename G, typename I>
+__global__ __launch_bounds__(1024) void embed_small_kernel(const T* __restrict__ dout, long dstride, const I* __restrict__ ids, int n,
+                                                           unsigned rows, int D, int ls, int pieces, int own, float scale,
+                                                           G* __restrict__ grad) {
+  __shared__ unsigned short off[16][SMALL_ROWS];
+  __shared__ unsigned char key_of[SMALL_MAX];
+  __shared__ unsigned short token_of[SMALL_MAX];
+  __shared__ unsigned long long s_empty[SMALL_ROWS / 64];
+  __shared__ int sums[SMALL_ROWS / 64];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const unsigned block = blockIdx.x / (unsigned)pieces, r0 = block * own;
+  // (a wave takes SMALL_STEPS x 64 neighbouring tokens)
+  unsigned d[SMALL_STEPS];
+#pragma unroll
+  for (int s = 0; s < SMALL_STEPS; s++) {
+    const int t = (w * SMALL_STEPS + s) * 64 + lane;
+    const unsigned k = n > 0 ? emb_key(ids[min(t, n - 1)], rows) : rows;
+    d[s] = t < n && k < rows ? k - r0 : 0xffffffffu;           // (rows below r0 wrap around)
+  }
+  for (int i = tid; i < 16 * SMALL_ROWS; i += 1024) off[i / SMALL_ROWS][i % SMALL_ROWS] = 0;
+  __syncthreads();
+  unsigned long long same[SMALL_STEPS];
+#pragma unroll
+  for (int s = 0; s < SMALL_STEPS; s++) {
+    const bool in = d[s] < (unsigned)own;
+    same[s] = 0;
+    if (__ballot(in)) {
+      same[s] = emb_same_digit((int)(d[s] & (SMALL_ROWS - 1)), 8, in);
+      if (in && (same[s] & ((1ull << lane) - 1)) == 0) off[w][d[s]] += (unsigned short)__popcll(same[s]);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+  __syncthreads();
+  int upto = 0, sum = 0;                                       // (thread: row)
+  if (tid < SMALL_ROWS) {
+#pragma unroll
+    for (int q = 0; q < 16; q++) sum += off[q][tid];
+    upto = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int from = __shfl_up(upto, o, 64);
+      upto += lane >= o ? from : 0;
+    }
+    const unsigned long long empty = __ballot(sum == 0 && tid < own && r0 + tid < rows);
+    if (lane == 0) s_empty[w] = empty;
+    if (lane == 63) sums[w] = upto;
+  }
+  __syncthreads();
+  int found = 0;
+#pragma unroll
+  for (int q = 0; q < SMALL_ROWS / 64; q++) found += sums[q];
+  if (tid < SMALL_ROWS) {
+    int at = upto - sum;
+#pragma unroll
+    for (int q = 0; q < SMALL_ROWS / 64; q++) at += q < w ? sums[q] : 0;
+#pragma unroll
+    for (int q = 0; q < 16; q++) {
+      const int c = off[q][tid];
+      off[q][tid] = (unsigned short)at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < SMALL_STEPS; s++) {
+    const bool in = d[s] < (unsigned)own;
+    const int before = __popcll(same[s] & ((1ull << lane) - 1));
+    const int p = in ? off[w][d[s]] : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in && before == 0) off[w][d[s]] = (unsigned short)(p + __popcll(same[s]));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (in) {
+      key_of[p + before] = (unsigned char)d[s];
+      token_of[p + before] = (unsigned short)((w * SMALL_STEPS + s) * 64 + lane);
+    }
+  }
+  __syncthreads();
+  const int first = (int)(blockIdx.x - block * pieces) * (V << ls) + (tid & ((1 << ls) - 1)) * V, c = min(first, D - V);
+  const bool col = first < D;
+  auto store = [&](unsigned r, float* acc) {
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] *= scale;
+    if (col) row_put<G, V, true>(grad + ((long)r0 + r) * D + c, acc);
+  };
+  for (int r = tid >> ls; r < own; r += 1024 >> ls)
+    if ((s_empty[r / 64] >> (r % 64)) & 1) {
+      float z[V];
+#pragma unroll
+      for (int i = 0; i < V; i++) z[i] = 0.0f;
+      if (col) row_put<G, V, true>(grad + ((long)r0 + r) * D + c, z);        // (0 whatever the scale)
+    }
+  const int groups = 1024 >> ls;
+  if (found == 0) return;
+  emb_sum_share<T, V, 16>(
+      dout + c, dstride, 0, found, SMALL_ROWS, ls, (found + groups - 1) / groups, [&](int p) { return (unsigned)key_of[p]; },
+      [&](int p) { return (int)token_of[p]; }, store, [](float*) {}, [](float*) {});
+}
+
+// ---------------------------------------------------------------------------------------------
 // C ABI
 // ---------------------------------------------------------------------------------------------
-// limits that keep every grid below 2^32 threads (up to 64 lanes per token, 8 per table row) and places in 32 bits
+// limits that keep every grid below 2^32 threads (up to 64 lanes per token, 16 per table row and piece of its columns) and places in
+// 32 bits
 #define EMB_MAX_COLS 65536
 #define EMB_MAX_TOKENS (1L << 25)
-#define EMB_MAX_ROWS (1L << 29)
+#define EMB_MAX_ROW_PIECES (1L << 27)     // rows x ceil(columns / 256) of a gradient
 
+// small: group = rows per workgroup, shares = pieces of the columns
 struct EmbPlan {
-  bool ranked, few;
+  bool small, ranked, few;
   int passes, bits, tiles, ls, group, shares;
   size_t keys[2], order[2], hist, total, part, touched, bytes;
 };
 
 static EmbPlan emb_plan(long n, long rows, int cols, int vec) {
   EmbPlan p = {};
+  p.ls = row_lanes_log2(cols, vec);
+  if (n <= SMALL_MAX) {
+    // narrow pieces of the columns: a row that takes most of the tokens is still the work of several workgroups
+    const int ls = p.ls < SMALL_LANES ? p.ls : SMALL_LANES, pieces = (cols + (vec << ls) - 1) / (vec << ls);
+    int own = 1;                                             // rows per workgroup
+    while (own < SMALL_ROWS && (rows + own - 1) / own * pieces > SMALL_BLOCKS) own *= 2;
+    if (n == 0 || (rows + own - 1) / own * pieces <= 4 * SMALL_BLOCKS) {
+      p.small = true;
+      p.ls = ls;
+      p.group = own;
+      p.shares = pieces;
+      return p;
+    }
+  }
   p.ranked = n <= RANK_MAX;
   int need = 1;
   while (need < 32 && ((unsigned long)rows >> need) != 0) need++;         // keys 0 .. rows
   p.passes = p.ranked ? 0 : (need + 9) / 10;
   p.bits = p.ranked ? 0 : (need + p.passes - 1) / p.passes;
   p.tiles = (int)((n + TILE - 1) / TILE);
-  p.ls = row_lanes_log2(cols, vec);
   const long lanes = n * (((cols + vec - 1) / vec + (1 << p.ls) - 1) >> p.ls << p.ls);       // lanes at one place per group
   p.group = GROUP;
   while (p.group < 128 && lanes / p.group > 64L * GROUP_WAVES) p.group *= 2;
@@ -831,6 +960,10 @@ static int emb_vec(int dtype, int D) {
   return D >= v ? v : 1;
 }
 
+static bool emb_fits(long n, long rows, int cols) {
+  return n <= EMB_MAX_TOKENS && cols >= 1 && cols <= EMB_MAX_COLS && rows <= EMB_MAX_ROW_PIECES / ((cols + 255) / 256);
+}
+
 static inline bool emb_type(int dtype) { return dtype == NS_F16 || dtype == NS_BF16 || dtype == NS_F32; }
 
 template <typename T, int V, typename I>
@@ -847,8 +980,8 @@ extern "C" int ns_embedding_forward(const void* table, long table_stride, const 
   NS_REQUIRE(emb_type(dtype), "ns_embedding_forward: dtype %d is not NS_F16, NS_BF16 or NS_F32", dtype);
   if (n == 0) return NS_OK;
   NS_REQUIRE(ids && out && (table || rows == 0), "ns_embedding_forward: null pointer");
-  NS_REQUIRE(n <= EMB_MAX_TOKENS && rows <= EMB_MAX_ROWS && cols >= 1 && cols <= EMB_MAX_COLS && table_stride >= 0,
-             "ns_embedding_forward: bad shape (n %ld <= 2^25, rows %ld <= 2^29, cols %d in 1 .. %d)", n, rows, cols, EMB_MAX_COLS);
+  NS_REQUIRE(n <= EMB_MAX_TOKENS && rows <= 0x7fffffffL && cols >= 1 && cols <= EMB_MAX_COLS && table_stride >= 0,
+             "ns_embedding_forward: bad shape (n %ld <= 2^25, rows %ld < 2^31, cols %d in 1 .. %d)", n, rows, cols, EMB_MAX_COLS);
   hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto t) {
     using T = decltype(t);
@@ -866,7 +999,7 @@ extern "C" int ns_embedding_forward(const void* table, long table_stride, const 
 }
 
 extern "C" size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols, int dtype) {
-  if (n <= 0 || n > EMB_MAX_TOKENS || rows < 0 || rows > EMB_MAX_ROWS || cols < 1 || cols > EMB_MAX_COLS) return 0;
+  if (n <= 0 || rows <= 0 || !emb_fits(n, rows, cols)) return 0;
   return emb_plan(n, rows, cols, emb_vec(dtype, cols)).bytes;
 }
 
@@ -907,6 +1040,13 @@ static void emb_sort(const EmbPlan& p, const I* ids, char* ws, int n, unsigned r
 }
 
 template <typename T, int V, typename G, typename I>
+static void emb_small(const EmbPlan& p, const T* dout, long dstride, const I* ids, int n, unsigned rows, int cols, float scale, G* grad,
+                      hipStream_t s) {
+  hipLaunchKernelGGL((embed_small_kernel<T, V, G, I>), dim3((rows + p.group - 1) / p.group * p.shares), dim3(1024), 0, s, dout, dstride, ids, n,
+                     rows, cols, p.ls, p.shares, p.group, scale, grad);
+}
+
+template <typename T, int V, typename G, typename I>
 static void emb_few(const EmbPlan& p, const T* dout, long dstride, const I* ids, int n, unsigned rows, int cols, float scale, G* grad,
                     char* ws, hipStream_t s) {
   float* part = (float*)(ws + p.part);
@@ -939,16 +1079,17 @@ extern "C" int ns_embedding_backward(const void* dout, long dout_stride, int dty
   NS_REQUIRE(emb_type(dtype) && (grad_dtype == dtype || grad_dtype == NS_F32),
              "ns_embedding_backward: dtype %d / grad dtype %d: NS_F16, NS_BF16 or NS_F32, and the gradient that or NS_F32", dtype, grad_dtype);
   if (rows == 0) return NS_OK;
-  NS_REQUIRE(grad && (n == 0 || (dout && ids && ws)), "ns_embedding_backward: null pointer");
-  NS_REQUIRE(n <= EMB_MAX_TOKENS && rows <= EMB_MAX_ROWS && cols >= 1 && cols <= EMB_MAX_COLS && dout_stride >= 0,
-             "ns_embedding_backward: bad shape (n %ld <= 2^25, rows %ld <= 2^29, cols %d in 1 .. %d)", n, rows, cols, EMB_MAX_COLS);
+  NS_REQUIRE(emb_fits(n, rows, cols) && dout_stride >= 0,
+             "ns_embedding_backward: bad shape (n %ld <= 2^25, cols %d in 1 .. %d, rows %ld x ceil(cols / 256) <= 2^27)", n, cols, EMB_MAX_COLS,
+             rows);
   const EmbPlan p = emb_plan(n, rows, cols, emb_vec(dtype, cols));
-  NS_REQUIRE(n == 0 || ws_bytes >= p.bytes, "ns_embedding_backward: workspace of %zu bytes, %zu needed", ws_bytes, p.bytes);
+  NS_REQUIRE(grad && (n == 0 || (dout && ids)) && (ws || p.bytes == 0), "ns_embedding_backward: null pointer");
+  NS_REQUIRE(ws_bytes >= p.bytes, "ns_embedding_backward: workspace of %zu bytes, %zu needed", ws_bytes, p.bytes);
   NS_REQUIRE(((uintptr_t)ws % 16) == 0, "ns_embedding_backward: the workspace needs 16-byte alignment");
   hipStream_t s = (hipStream_t)stream;
   const unsigned* keys = nullptr;
   const int* order = nullptr;
-  if (n > 0 && !p.few) {
+  if (!p.small && !p.few) {
     if (ids_are_64) emb_sort(p, (const int64_t*)ids, (char*)ws, (int)n, (unsigned)rows, &keys, &order, s);
     else emb_sort(p, (const int32_t*)ids, (char*)ws, (int)n, (unsigned)rows, &keys, &order, s);
     NS_CHECK_LAUNCH("embedding_backward: sort");
@@ -958,11 +1099,19 @@ extern "C" int ns_embedding_backward(const void* dout, long dout_stride, int dty
     float* part = (float*)((char*)ws + p.part);
     emb_pieces<T>(cols, [&](auto piece) {
       constexpr int V = decltype(piece)::v;
+      auto small = [&](auto* g) {
+        if (ids_are_64) emb_small<T, V>(p, (const T*)dout, dout_stride, (const int64_t*)ids, (int)n, (unsigned)rows, cols, scale, g, s);
+        else emb_small<T, V>(p, (const T*)dout, dout_stride, (const int32_t*)ids, (int)n, (unsigned)rows, cols, scale, g, s);
+      };
       auto few = [&](auto* g) {
         if (ids_are_64) emb_few<T, V>(p, (const T*)dout, dout_stride, (const int64_t*)ids, (int)n, (unsigned)rows, cols, scale, g, (char*)ws, s);
         else emb_few<T, V>(p, (const T*)dout, dout_stride, (const int32_t*)ids, (int)n, (unsigned)rows, cols, scale, g, (char*)ws, s);
       };
-      if (p.few && grad_dtype == NS_F32)
+      if (p.small && grad_dtype == NS_F32)
+        small((float*)grad);
+      else if (p.small)
+        small((T*)grad);
+      else if (p.few && grad_dtype == NS_F32)
         few((float*)grad);
       else if (p.few)
         few((T*)grad);

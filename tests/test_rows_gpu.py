@@ -122,7 +122,8 @@ def check_grad(got, dout, ids, v, scale, what):
     within(got, want, tol, what)
 
 
-SIZES = [(1, 1, 1), (1, 40, 16), (15, 3, 5), (16, 3, 8), (17, 3, 8), (33, 1000, 33), (64, 7, 771), (300, 2, 1030), (1000, 64, 32),
+SIZES = [(1, 1, 1), (1, 40, 16), (15, 3, 5), (16, 3, 8), (17, 3, 8), (33, 1000, 33), (64, 7, 771), (300, 2, 1030), (1000, 64, 32), (1023, 300, 40), (1024, 70000, 6), (1025, 1, 64), (4095, 257, 130), (4096, 20000, 17),
+         (5000, 7, 12), (6001, 900, 771),
          (8192, 300, 8), (8193, 300, 8), (8193, 1023, 4), (9000, 1024, 12), (20000, 70000, 3), (40000, 5, 16), (4097, 5000, 2050),
          (8200, 512, 33), (9300, 512, 64), (30000, 64, 3), (12345, 1, 31), (10240, 513, 32), (9100, 1023, 20), (9200, 1024, 20)]
 
@@ -153,7 +154,7 @@ def test_embedding_backward_sorts_stably(dev):
     """integers sum exactly in f32 whatever the order; 2^24-sized ones do not: a fixed order gives the same bits on every call, and an
     exact case gives exact sums for every row of a long skewed list"""
     g = gen(dev, 5)
-    for n in (5000, 100000):
+    for n in (700, 5000, 20000, 100000):
         ids = make_ids(g, n, 3000, "skew")
         whole = torch.randint(-8, 9, (n, 24), generator=g, device=dev).to(F16)
         want = torch.zeros((3000, 24), dtype=torch.float64, device=dev).index_add_(0, ids, whole.double())
@@ -420,7 +421,7 @@ def _chain(table, ids, w, b, c, v):
     return y, dw, db, rows.embedding_backward(de, ids, v, scale=2.0)
 
 
-@pytest.mark.parametrize("n,v", [(300, 40), (9000, 2000)])
+@pytest.mark.parametrize("n,v", [(300, 40), (5000, 30), (9000, 2000), (9000, 200), (40000, 3000)])
 def test_captured_and_replayed(dev, n, v):
     """a whole pass in one HIP graph, replayed on new inputs with eager calls and synchronizations in between; two graphs, each with
     its own workspaces, replayed in turn"""
@@ -472,7 +473,7 @@ def test_nothing_is_written_outside_the_outputs(dev):
     g = gen(dev, 13)
     f = lib()
     L = C.c_long
-    for n, v, d in ((37, 11, 33), (9000, 700, 5), (70, 300, 520)):
+    for n, v, d in ((37, 11, 33), (9000, 700, 5), (70, 300, 520), (5000, 70, 33), (20000, 2000, 70)):
         ids = make_ids(g, n, v, "pad", torch.int32)
         x = randn(g, n * d + 1, dtype=F16)[1:]                                  # 2-byte alignment
         table = randn(g, v * d + 1, dtype=F16)[1:]

@@ -71,19 +71,21 @@ def test_abi_refusals():
     _refused(f.ns_embedding_forward(P, L(-1), P, 0, P, 1, L(3), L(5), 4, C.c_float(1), None), "bad shape")
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(-3), L(5), 4, C.c_float(1), None), "bad shape")
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L((1 << 25) + 1), L(5), 4, C.c_float(1), None), "2^25")
-    _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(3), L((1 << 29) + 1), 4, C.c_float(1), None), "2^29")
+    _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(3), L(1 << 31), 4, C.c_float(1), None), "2^31")
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(3), L(5), 0, C.c_float(1), None), "bad shape")
     _refused(f.ns_embedding_forward(P, L(4), P, 0, P, 1, L(3), L(5), 65537, C.c_float(1), None), "65536")
     assert f.ns_embedding_forward(None, L(4), None, 0, None, 1, L(0), L(5), 4, C.c_float(1), None) == 0        # nothing to do
 
     big = C.c_size_t(1 << 40)
     _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, None, 1, L(3), L(5), 4, C.c_float(1), P, big, None), "null pointer")
-    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(3), L(5), 4, C.c_float(1), None, big, None), "null pointer")
+    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(50000), L(5), 4, C.c_float(1), None, big, None), "null pointer")
     _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 3, L(3), L(5), 4, C.c_float(1), P, big, None), "grad dtype")
     _refused(f.ns_embedding_backward(P, L(4), 2, P, 0, P, 1, L(3), L(5), 4, C.c_float(1), P, big, None), "grad dtype")
-    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(3), L(5), 4, C.c_float(1), P, z, None), "workspace")
+    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(50000), L(5), 4, C.c_float(1), P, z, None), "workspace")
     _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(3), L(5), 4, C.c_float(1), C.c_void_p(4100), big, None), "alignment")
     _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L((1 << 25) + 1), L(5), 4, C.c_float(1), P, big, None), "2^25")
+    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(3), L((1 << 27) + 1), 4, C.c_float(1), P, big, None), "2^27")
+    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(3), L((1 << 26) + 1), 257, C.c_float(1), P, big, None), "2^27")
     assert f.ns_embedding_backward(None, L(4), 1, None, 0, None, 1, L(3), L(0), 4, C.c_float(1), None, z, None) == 0
 
     e = C.c_float(1e-5)
@@ -108,7 +110,8 @@ def test_workspace_sizes():
     f = lib()
     emb, ln = f.ns_embedding_backward_workspace_bytes, f.ns_layer_norm_backward_workspace_bytes
     assert emb(L(0), L(5), 4, 1) == 0 and ln(L(0), 4, 2) == 0
-    for n in (1, 17, 8192, 8193, 1 << 20):
+    assert emb(L(1), L(1000), 64, 2) == 0                    # (short lists need none)
+    for n in (8192, 8193, 1 << 20):
         assert emb(L(n), L(1000), 64, 2) >= 8 * n and emb(L(n), L(1000), 64, 3) % 16 == 0
-    assert emb(L(1 << 25), L(1 << 29), 65536, 1) > 2 ** 31          # (no 32-bit arithmetic in it)
+    assert emb(L(1 << 25), L(1 << 19), 65536, 1) > 2 ** 31          # (no 32-bit arithmetic in it)
     assert ln(L(10), 64, 2) % 512 == 0 and ln(L(1 << 20), 64, 2) > 0
