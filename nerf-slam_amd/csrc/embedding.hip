@@ -43,6 +43,9 @@
 #define FEW_LANES 3
 #endif
 #define FEW_TILES 1024
+#ifndef FEW_WAVES
+#define FEW_WAVES 8
+#endif
 #ifndef SMALL_MAX
 #define SMALL_MAX 4096       // tokens up to which the gradient is one launch
 #endif
@@ -368,11 +371,13 @@ __global__ __launch_bounds__(TILE) void embed_pass_kernel(const I* __restrict__ 
     int at = upto - mine + prior;
 #pragma unroll
     for (int i = 0; i < ONE_WAVES; i++) at += i < w ? part[i] : 0;
+    int c[ONE_WAVES];
+#pragma unroll
+    for (int i = 0; i < ONE_WAVES; i++) c[i] = off[i * bins + tid];
 #pragma unroll
     for (int i = 0; i < ONE_WAVES; i++) {
-      const int c = off[i * bins + tid];
       off[i * bins + tid] = (unsigned short)at;
-      at += c;
+      at += c[i];
     }
   }
   __syncthreads();
@@ -650,21 +655,21 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const unsigned* __restr
 // touched [tiles][32]; then a workgroup per row adds the tiles' sums in order.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int V, typename I>
-__global__ __launch_bounds__(256) void embed_tile_kernel(const T* __restrict__ dout, long dstride, const I* __restrict__ ids, int n,
+__global__ __launch_bounds__(64 * FEW_WAVES) void embed_tile_kernel(const T* __restrict__ dout, long dstride, const I* __restrict__ ids, int n,
                                                          unsigned rows, int D, int ls, int tiles, float* __restrict__ part,
                                                          unsigned* __restrict__ touched) {
-  __shared__ int off[4][MAX_BINS];
+  __shared__ __align__(4) unsigned short off[FEW_WAVES][MAX_BINS];
   __shared__ unsigned short key_of[TILE], token_of[TILE];
   __shared__ unsigned bits[MAX_BINS / 32];
-  __shared__ int sums[4];
-  constexpr int STEPS = TILE / 256, PER = MAX_BINS / 256;
+  __shared__ int sums[FEW_WAVES];
+  constexpr int THREADS = 64 * FEW_WAVES, STEPS = TILE / THREADS, PER = MAX_BINS / THREADS;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int tile = blockIdx.x;
   const int t0 = tile * TILE, have = min(n - t0, TILE);
   unsigned key[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; s++) key[s] = emb_key(ids[t0 + min((w * STEPS + s) * 64 + lane, have - 1)], rows);
-  for (int i = tid; i < 4 * MAX_BINS; i += 256) off[i / MAX_BINS][i % MAX_BINS] = 0;
+  for (int i = tid; i < FEW_WAVES * MAX_BINS / 2; i += THREADS) reinterpret_cast<unsigned*>(off)[i] = 0;
   if (tid < MAX_BINS / 32) bits[tid] = 0;
   __syncthreads();
   unsigned long long same[STEPS];
@@ -672,15 +677,20 @@ __global__ __launch_bounds__(256) void embed_tile_kernel(const T* __restrict__ d
   for (int s = 0; s < STEPS; s++) {
     const bool in = (w * STEPS + s) * 64 + lane < have;
     same[s] = emb_same_digit((int)key[s], MAX_BITS, in);
-    if (in && (same[s] & ((1ull << lane) - 1)) == 0) off[w][key[s]] += __popcll(same[s]);
+    if (in && (same[s] & ((1ull << lane) - 1)) == 0) off[w][key[s]] += (unsigned short)__popcll(same[s]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   __syncthreads();
-  int tot[PER], sum = 0;                                       // (thread: PER neighbouring rows)
+  int tot[PER], cnt[PER][FEW_WAVES], sum = 0;                                       // (thread: PER neighbouring rows)
   unsigned seen = 0;
 #pragma unroll
   for (int i = 0; i < PER; i++) {
-    tot[i] = off[0][tid * PER + i] + off[1][tid * PER + i] + off[2][tid * PER + i] + off[3][tid * PER + i];
+    tot[i] = 0;
+#pragma unroll
+    for (int q = 0; q < FEW_WAVES; q++) {
+      cnt[i][q] = off[q][tid * PER + i];
+      tot[i] += cnt[i][q];
+    }
     seen |= tot[i] ? 1u << i : 0u;
     sum += tot[i];
   }
@@ -695,14 +705,13 @@ __global__ __launch_bounds__(256) void embed_tile_kernel(const T* __restrict__ d
   __syncthreads();
   int at = upto - sum;
 #pragma unroll
-  for (int i = 0; i < 3; i++) at += i < w ? sums[i] : 0;
+  for (int i = 0; i < FEW_WAVES - 1; i++) at += i < w ? sums[i] : 0;
 #pragma unroll
   for (int i = 0; i < PER; i++)
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const int c = off[q][tid * PER + i];
-      off[q][tid * PER + i] = at;
-      at += c;
+    for (int q = 0; q < FEW_WAVES; q++) {
+      off[q][tid * PER + i] = (unsigned short)at;
+      at += cnt[i][q];
     }
   __syncthreads();
 #pragma unroll
@@ -712,7 +721,7 @@ __global__ __launch_bounds__(256) void embed_tile_kernel(const T* __restrict__ d
     const int before = __popcll(same[s] & ((1ull << lane) - 1));
     const int p = in ? off[w][key[s]] : 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (in && before == 0) off[w][key[s]] = p + __popcll(same[s]);
+    if (in && before == 0) off[w][key[s]] = (unsigned short)(p + __popcll(same[s]));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (in) {
       key_of[p + before] = (unsigned short)key[s];
@@ -727,8 +736,8 @@ __global__ __launch_bounds__(256) void embed_tile_kernel(const T* __restrict__ d
     if (col) row_put<float, V, false>(part + ((long)r * tiles + tile) * D + c, acc);
   };
   // (nothing enters or leaves: the share is the whole list)
-  emb_sum_share<T, V, 4>(
-      dout + (long)t0 * dstride + c, dstride, 0, have, rows, ls, (TILE / 256) << ls, [&](int p) { return (unsigned)key_of[p]; },
+  emb_sum_share<T, V, FEW_WAVES>(
+      dout + (long)t0 * dstride + c, dstride, 0, have, rows, ls, STEPS << ls, [&](int p) { return (unsigned)key_of[p]; },
       [&](int p) { return (int)token_of[p]; }, store, [](float*) {}, [](float*) {});
 }
 
@@ -831,14 +840,15 @@ __global__ __launch_bounds__(1024) void embed_small_kernel(const T* __restrict__
 #pragma unroll
   for (int q = 0; q < SMALL_ROWS / 64; q++) found += sums[q];
   if (tid < SMALL_ROWS) {
-    int at = upto - sum;
+    int at = upto - sum, c[16];
 #pragma unroll
     for (int q = 0; q < SMALL_ROWS / 64; q++) at += q < w ? sums[q] : 0;
 #pragma unroll
+    for (int q = 0; q < 16; q++) c[q] = off[q][tid];
+#pragma unroll
     for (int q = 0; q < 16; q++) {
-      const int c = off[q][tid];
       off[q][tid] = (unsigned short)at;
-      at += c;
+      at += c[q];
     }
   }
   __syncthreads();
@@ -1051,7 +1061,7 @@ static void emb_few(const EmbPlan& p, const T* dout, long dstride, const I* ids,
                     char* ws, hipStream_t s) {
   float* part = (float*)(ws + p.part);
   unsigned* touched = (unsigned*)(ws + p.touched);
-  hipLaunchKernelGGL((embed_tile_kernel<T, V, I>), dim3(p.tiles), dim3(256), 0, s, dout, dstride, ids, n, rows, cols, p.ls, p.tiles, part,
+  hipLaunchKernelGGL((embed_tile_kernel<T, V, I>), dim3(p.tiles), dim3(64 * FEW_WAVES), 0, s, dout, dstride, ids, n, rows, cols, p.ls, p.tiles, part,
                      touched);
   hipLaunchKernelGGL((embed_rows_kernel<G, V>), dim3(rows), dim3(256), 0, s, part, touched, p.tiles, cols, p.ls, scale, grad);
 }

@@ -113,14 +113,14 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T
 }
 
 // ---------------------------------------------------------------------------------------------
-// backward.  part: [workgroups][2][D] f32 (dw | db), or nullptr: no weight.
+// backward.  part: [workgroups][2][D] f32 (dw | db); a single workgroup writes dweight and dbias itself (no weight: nobody).
 // ---------------------------------------------------------------------------------------------
 template <typename T, typename W, int LPR, int NV>
 __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T* __restrict__ dy, long dstride, const T* __restrict__ x,
                                                                          long xstride, const float* __restrict__ mean,
                                                                          const float* __restrict__ rstd, const W* __restrict__ w,
-                                                                         T* __restrict__ dx, float* __restrict__ part, long n, int D,
-                                                                         float inv_d) {
+                                                                         T* __restrict__ dx, float* __restrict__ part, W* __restrict__ dweight,
+                                                                         W* __restrict__ dbias, long n, int D, float inv_d) {
   constexpr int V = row_vec<T>(), BLOCK = ln_block<LPR>(), ROWS = BLOCK / LPR;
   __shared__ float red[2][LPR > 64 ? LPR / 64 : 1][2];
   __shared__ float cols[ROWS > 1 ? BLOCK * (V + 1) : 1];
@@ -186,8 +186,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
       row_store<T, V>(dx + r * D, (j * LPR + lane) * V, D, f);
     }
   }
-  if (!part) return;
-  float* mine = part + (long)blockIdx.x * 2 * D;
+  if (!w) return;
 #pragma unroll
   for (int k = 0; k < 2; k++)
 #pragma unroll
@@ -205,7 +204,10 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
             for (int i = 0; i < V; i++) acc[i] += cols[(t * LPR + lane) * (V + 1) + i];
         }
       }
-      if (threadIdx.x < LPR) row_store<float, V>(mine + (long)k * D, (j * LPR + lane) * V, D, acc);
+      if (threadIdx.x < LPR) {
+        if (gridDim.x == 1) row_store<W, V>(k ? dbias : dweight, (j * LPR + lane) * V, D, acc);
+        else row_store<float, V>(part + ((long)blockIdx.x * 2 + k) * D, (j * LPR + lane) * V, D, acc);
+      }
     }
 }
 
@@ -252,7 +254,7 @@ static void ln_shape(int D, F f) {
   else if (pieces <= 256) f(LnInt<256>(), LnInt<1>());
   else if (pieces <= 512) f(LnInt<256>(), LnInt<2>());
   else if (pieces <= 1024) f(LnInt<(BACK ? 512 : 256)>(), LnInt<(BACK ? 2 : 4)>());
-  else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
+    else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
   else if constexpr (V == 4) f(LnInt<1024>(), LnInt<4>());
 }
 
@@ -317,7 +319,8 @@ extern "C" int ns_layer_norm_forward(const void* x, long x_stride, const void* w
 
 extern "C" size_t ns_layer_norm_backward_workspace_bytes(long n, int cols, int dtype) {
   if (n <= 0 || cols < 1 || cols > LN_MAX_COLS) return 0;
-  return (size_t)ln_blocks(n, cols, dtype == NS_F32 ? 4 : 8, true) * 2 * cols * 4;
+  const int blocks = ln_blocks(n, cols, dtype == NS_F32 ? 4 : 8, true);
+  return blocks > 1 ? (size_t)blocks * 2 * cols * 4 : 0;
 }
 
 extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void* x, long x_stride, const float* mean, const float* rstd,
@@ -338,10 +341,10 @@ extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void
       ln_shape<row_vec<T>(), true>(cols, [&](auto lpr, auto nv) {
         constexpr int L = decltype(lpr)::v, N = decltype(nv)::v;
         hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, L, N>), dim3(blocks), dim3(ln_block<L>()), 0, (hipStream_t)stream, (const T*)dy,
-                           dy_stride, (const T*)x, x_stride, mean, rstd, (const W*)weight, (T*)dx, weight ? (float*)ws : nullptr, n, cols,
+                           dy_stride, (const T*)x, x_stride, mean, rstd, (const W*)weight, (T*)dx, (float*)ws, (W*)dweight, (W*)dbias, n, cols,
                            1.0f / (float)cols);
       });
-    if (weight)
+    if (weight && blocks != 1)                                 // (0 workgroups, no rows: zeros)
       hipLaunchKernelGGL(layer_norm_wgrad_kernel<W>, dim3((2 * cols + 63) / 64), dim3(1024), 0, (hipStream_t)stream, (const float*)ws, blocks,
                          cols, (W*)dweight, (W*)dbias);
   });

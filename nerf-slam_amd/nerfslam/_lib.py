@@ -50,7 +50,9 @@ def _load(path):
     L.ns_ba_solve_large_workspace_bytes.restype = C.c_size_t
     L.ns_ngp_mlp_fragment_table_bytes.restype = C.c_size_t
     L.ns_embedding_backward_workspace_bytes.restype = C.c_size_t
+    L.ns_embedding_backward_workspace_bytes.argtypes = [C.c_long, C.c_long, C.c_int, C.c_int]
     L.ns_layer_norm_backward_workspace_bytes.restype = C.c_size_t
+    L.ns_layer_norm_backward_workspace_bytes.argtypes = [C.c_long, C.c_int, C.c_int]
     return L
 
 

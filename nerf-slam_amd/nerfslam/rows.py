@@ -8,6 +8,7 @@ explicit, as the trainer's are: nothing here records on torch's autograd tape.  
 device, nothing synchronises, and every call has its own workspace, so calls may be captured into HIP graphs and run on several streams.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -21,10 +22,13 @@ def _fail(op, what):
 
 
 def _same_device(op, first, *others):
-    require_cuda(first, *others)
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.device != device:
+            require_cuda(first, *others)
             _fail(op, "all tensors have to be on one device")
+    require_cuda(first)
+    return device
 
 
 def _call(name, what, device, *args):
@@ -34,6 +38,12 @@ def _call(name, what, device, *args):
             return _call(name, what, device, *args)
     # (the stream's handle without building torch's Stream object: 0.1 us instead of 3.4, of calls that take 3 us on the device)
     check(getattr(lib(), name)(*args, C.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))), what)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, n, *args):
+    """what a size query of the library answers: a function of sizes alone"""
+    return getattr(lib(), name)(n, *args)
 
 
 def _rows_of(op, name, t):
@@ -79,11 +89,11 @@ def embedding(table, ids, scale=1.0):
         _fail("embedding", "the table is a [rows, D] tensor")
     rows, stride = _rows_of("embedding", "table", table)
     is64 = _ids("embedding", ids)
-    _same_device("embedding", table, ids)
+    device = _same_device("embedding", table, ids)
     cols = table.shape[1]
     out = table.new_empty((*ids.shape, cols))
     if out.numel():
-        _call("ns_embedding_forward", "embedding_forward", out.device, ptr(table), C.c_long(stride), ptr(ids), is64, ptr(out),
+        _call("ns_embedding_forward", "embedding_forward", device, ptr(table), C.c_long(stride), ptr(ids), is64, ptr(out),
               _DT[table.dtype], C.c_long(ids.numel()), C.c_long(rows), cols, C.c_float(scale))
     return out
 
@@ -103,12 +113,12 @@ def embedding_backward(dout, ids, rows, scale=1.0, dtype=None):
     rows, cols = int(rows), dout.shape[-1]
     if rows < 0:
         _fail(op, f"{rows} rows")
-    _same_device(op, dout, ids)
-    grad = dout.new_empty((rows, cols), dtype=dtype)
+    device = _same_device(op, dout, ids)
+    grad = torch.empty((rows, cols), dtype=dtype, device=device)
     if grad.numel():
-        nbytes = lib().ns_embedding_backward_workspace_bytes(C.c_long(n), C.c_long(rows), cols, _DT[dout.dtype])
-        ws = dout.new_empty(nbytes, dtype=torch.uint8)
-        _call("ns_embedding_backward", op, grad.device, ptr(dout), C.c_long(stride), _DT[dout.dtype], ptr(ids), is64, ptr(grad), _DT[dtype],
+        nbytes = _workspace_bytes("ns_embedding_backward_workspace_bytes", n, rows, cols, _DT[dout.dtype])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _call("ns_embedding_backward", op, device, ptr(dout), C.c_long(stride), _DT[dout.dtype], ptr(ids), is64, ptr(grad), _DT[dtype],
               C.c_long(n), C.c_long(rows), cols, C.c_float(scale), ptr(ws), C.c_size_t(nbytes))
     return grad
 
@@ -135,12 +145,13 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=False):
         if weight is not None and bdtype != wdtype:
             _fail(op, "weight and bias have to be of one dtype")
         wdtype = bdtype
-    _same_device(op, x, weight, bias)
+    device = _same_device(op, x, weight, bias)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = None
     if stats:
-        mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
-    _call("ns_layer_norm_forward", "layer_norm_forward", x.device, ptr(x), C.c_long(stride), ptr(weight), ptr(bias), _DT[wdtype], ptr(y),
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+        rstd = torch.empty_like(mean)
+    _call("ns_layer_norm_forward", "layer_norm_forward", device, ptr(x), C.c_long(stride), ptr(weight), ptr(bias), _DT[wdtype], ptr(y),
           ptr(mean), ptr(rstd), _DT[x.dtype], C.c_long(n), x.shape[-1], C.c_float(eps))
     return (y, mean, rstd) if stats else y
 
@@ -157,15 +168,15 @@ def layer_norm_backward(dout, x, mean, rstd, weight=None):
         if t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous():
             _fail(op, f"{name} must be a contiguous float32 {tuple(x.shape[:-1])} tensor")
     wdtype = torch.float32 if weight is None else _weight(op, x, "weight", weight)
-    _same_device(op, x, dout, mean, rstd, weight)
+    device = _same_device(op, x, dout, mean, rstd, weight)
     cols = x.shape[-1]
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = db = ws = None
     nbytes = 0
     if weight is not None:
         dw, db = torch.empty_like(weight), torch.empty_like(weight)
-        nbytes = lib().ns_layer_norm_backward_workspace_bytes(C.c_long(n), cols, _DT[x.dtype])
-        ws = x.new_empty(nbytes, dtype=torch.uint8)
-    _call("ns_layer_norm_backward", op, x.device, ptr(dout), C.c_long(dstride), ptr(x), C.c_long(stride), ptr(mean), ptr(rstd), ptr(weight),
+        nbytes = _workspace_bytes("ns_layer_norm_backward_workspace_bytes", n, cols, _DT[x.dtype])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _call("ns_layer_norm_backward", op, device, ptr(dout), C.c_long(dstride), ptr(x), C.c_long(stride), ptr(mean), ptr(rstd), ptr(weight),
           _DT[wdtype], ptr(dx), ptr(dw), ptr(db), _DT[x.dtype], C.c_long(n), cols, ptr(ws), C.c_size_t(nbytes))
     return dx, dw, db

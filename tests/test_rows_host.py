@@ -101,7 +101,7 @@ def test_abi_refusals():
 
     _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, None, P, 2, P, P, P, 2, L(3), 4, P, big, None), "null pointer")
     _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, P, P, 2, P, None, P, 2, L(3), 4, P, big, None), "together")
-    _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, P, P, 2, P, P, P, 2, L(3), 4, P, z, None), "workspace")
+    _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, P, P, 2, P, P, P, 2, L(3000), 4, P, z, None), "workspace")
     _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, P, P, 2, P, P, P, 2, L(3), 0, P, big, None), "bad shape")
     _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, P, P, 3, P, P, P, 2, L(3), 4, P, big, None), "weight dtype")
 
@@ -114,4 +114,4 @@ def test_workspace_sizes():
     for n in (8192, 8193, 1 << 20):
         assert emb(L(n), L(1000), 64, 2) >= 8 * n and emb(L(n), L(1000), 64, 3) % 16 == 0
     assert emb(L(1 << 25), L(1 << 19), 65536, 1) > 2 ** 31          # (no 32-bit arithmetic in it)
-    assert ln(L(10), 64, 2) % 512 == 0 and ln(L(1 << 20), 64, 2) > 0
+    assert ln(L(1), 64, 2) == 0 and ln(L(1000), 64, 2) % 512 == 0 and ln(L(1 << 20), 64, 2) > 0
