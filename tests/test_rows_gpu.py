@@ -125,7 +125,8 @@ def check_grad(got, dout, ids, v, scale, what):
 SIZES = [(1, 1, 1), (1, 40, 16), (15, 3, 5), (16, 3, 8), (17, 3, 8), (33, 1000, 33), (64, 7, 771), (300, 2, 1030), (1000, 64, 32), (1023, 300, 40), (1024, 70000, 6), (1025, 1, 64), (4095, 257, 130), (4096, 20000, 17),
          (5000, 7, 12), (6001, 900, 771),
          (8192, 300, 8), (8193, 300, 8), (8193, 1023, 4), (9000, 1024, 12), (20000, 70000, 3), (40000, 5, 16), (4097, 5000, 2050),
-         (8200, 512, 33), (9300, 512, 64), (30000, 64, 3), (12345, 1, 31), (10240, 513, 32), (9100, 1023, 20), (9200, 1024, 20)]
+         (8200, 512, 33), (9300, 512, 64), (30000, 64, 3), (12345, 1, 31), (10240, 513, 32), (9100, 1023, 20), (9200, 1024, 20),
+         (32768, 60000, 6), (32769, 60000, 6), (16385, 65535, 8), (16384, 65536, 8), (8195, 4000000, 9)]
 
 
 @pytest.mark.parametrize("kind", ["even", "skew", "pad"])
