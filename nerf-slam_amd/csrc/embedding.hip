@@ -5,57 +5,50 @@
 // An id outside [0, rows) is a padded place: its output row is zero and its upstream gradient is not read.
 //
 // The gradient is a sum over the tokens SORTED by id, without floating-point atomics: the order of every sum is fixed by the ids
-// alone, so the same inputs give the same bits.  The sort is stable; its sums run over equal shares of the sorted list instead of
-// over rows, so a row that a tenth of the tokens name costs no more than any other.
-//   1. sort   n <= RANK_MAX: one launch, a token's place counted directly (embed_rank_kernel); longer: radix passes of up to 10 bits, one
-//             launch each up to ONE_MAX tokens (embed_pass_kernel), beyond as histogram, prefix, scatter
-//   2. sums   a group of lanes walks GROUP consecutive places and sums runs of equal ids in f32 registers; a run inside the share
-//             is final, a run that crosses its ends leaves one f32 partial row per share
-//   3. join   the share in which a crossing run begins adds its partial rows in order (embed_join_kernel)
+// alone, so the same inputs give the same bits.  All sorts are stable.  Three forms, by sizes (times of one call on the device):
+//   short list   n <= SMALL_MAX: one launch; a workgroup owns neighbouring rows of the table and picks their tokens out of the whole list
+//                (embed_small_kernel; 3001 tokens of 771 f32, 1013 rows: 11 us)
+//   few rows     up to FEW_ROWS rows of up to 16 lanes: two launches; a workgroup sorts and sums a tile of tokens, then the tiles' sums are
+//                added per row (embed_tile_kernel, embed_rows_kernel; 262144 tokens of 32 f16, 512 rows: 14 us, 28 in the next form)
+//   general      sort, sums over equal shares of the sorted list -- so that a row that a tenth of the tokens name costs no more than any
+//                other --, join (16384 tokens of 1024 bf16, 50000 rows: 45 us = 3.0 TB/s of its 135 MB)
+//     sort   n <= RANK_MAX: one launch, a token's place counted directly (embed_rank_kernel); longer: radix passes of up to 10 bits, one
+//            launch each up to ONE_MAX tokens (embed_pass_kernel), beyond as histogram, prefix, scatter
+//     sums   a group of lanes walks consecutive places and sums runs of equal ids in f32 registers (emb_sum_share); a run inside the
+//            workgroup's share is final, one that crosses its ends leaves one f32 partial row per share (embed_sum_kernel, which also
+//            writes the rows without tokens)
+//     join   the share in which a crossing run begins adds its partial rows in order (embed_join_kernel)
+// The general form moves little more than dout and the gradient; beside them it is bound by the latency of its four or five launches,
+// each a chain of dependent loads (sort 20 us, sums 22, join 4 of the 45).
 //
 // Columns: a lane holds V of them, 16 bytes, or one where a row is shorter than 16 bytes.  The last piece of a row ends with the row, so
 // where D is no multiple of V it overlaps the one before: both lanes form the same sums in the same order and store the same bits.
+// Outputs are stored past the caches (16384 tokens / 50000 rows of 1024 bf16: 72 -> 58 us; lookup of 65536 tokens of 2048: 153 -> 87).
 #include "rows.h"
 
-#define RANK_MAX 8192        // tokens whose places are counted directly
-#ifndef ONE_MAX
-#define ONE_MAX 32768        // tokens up to which a radix pass is one launch
-#endif
-#define TILE 1024            // tokens per workgroup of a radix pass
-#ifndef GROUP
-#define GROUP 8              // places of the sorted list per group of lanes, doubled (to 128) while more than GROUP_WAVES waves are at work
-#endif
-#ifndef GROUP_WAVES
-#define GROUP_WAVES 2048
-#endif
-#ifndef ZERO_ROWS
-#define ZERO_ROWS 8         // table rows per wave that looks for rows without tokens
-#endif
-#ifndef SUM_U
-#define SUM_U 8
-#endif
+// ---- short list ----
+#define SMALL_MAX 4096       // tokens.  At 4096, 1000 rows: 8 us (32 columns) and 10 (1024) against 13 and 13 in the general form; all tokens
+                             // of one row: 12 and 21 against 12 and 25
+#define SMALL_ROWS 256       // most rows of the table per workgroup
+#define SMALL_BLOCKS 256     // workgroups aimed at -- one round on the chip; 512: 3001 tokens 17 us instead of 11 --, and a quarter of what is
+                             // allowed (beyond, the general form)
+#define SMALL_LANES 4        // log2 of the most lanes per row: a row that takes all of 4096 tokens of 1024 bf16 costs 21 us, with 64 lanes 55
+// ---- few rows ----
+#define FEW_ROWS (MAX_BINS - 1)   // 1000 rows, 262144 tokens of 64 f16 in random order: 28 us against 35 in the general form
+#define FEW_LANES 4          // log2 of the most lanes per row.  At 4 (128 f16, 262144 tokens): 24 against 33 us in runs of 64 equal ids, 42
+                             // against 37 in random order; 32768 tokens: 13 / 21 against 32 / 25.  At 5 random order loses everywhere
+#define FEW_TILES 1024       // 2^20 tokens: 46 against 71 us; bounds the workspace
+#define FEW_WAVES 8          // per tile; 4 or 16: 14.4 or 14.6 us instead of 13.6
+// ---- general ----
+#define RANK_MAX 8192        // 6000 / 8192 tokens: 19 / 22 us against 22 / 23 with radix passes; 16384: 61 against 51
+#define ONE_MAX 16384        // 16384 tokens, two passes: 51 us against 56 as three launches a pass; 32768: 44 against 41
+#define TILE 1024            // tokens per workgroup of a radix pass and of the few rows' form
 #define MAX_BITS 10          // of a radix pass' digit
 #define MAX_BINS (1 << MAX_BITS)
-#ifndef FEW_ROWS
-#define FEW_ROWS (MAX_BINS - 1)
-#endif
-#ifndef FEW_LANES
-#define FEW_LANES 3
-#endif
-#define FEW_TILES 1024
-#ifndef FEW_WAVES
-#define FEW_WAVES 8
-#endif
-#ifndef SMALL_MAX
-#define SMALL_MAX 4096       // tokens up to which the gradient is one launch
-#endif
-#define SMALL_ROWS 256       // ... and most rows of the table per workgroup there
-#ifndef SMALL_BLOCKS
-#define SMALL_BLOCKS 256     // workgroups that this form aims at, a quarter of what it takes at most
-#endif
-#ifndef SMALL_LANES
-#define SMALL_LANES 4
-#endif
+#define SUM_U 8              // rows that a lane has on their way; 16: 78 instead of 61 us at 65536 tokens of 512 (fewer waves fit), 4: equal
+#define GROUP 8              // places of the sorted list per group of lanes, doubled (up to 128) while more than GROUP_WAVES waves are
+#define GROUP_WAVES 2048     // at work.  4096 / 8192 waves: 55 / 54 instead of 49 us at 16384 tokens of 1024
+#define ZERO_ROWS 8          // table rows per wave that looks for rows without tokens; 32: 15.4 instead of 13.6 us at 3001 tokens, equal elsewhere
 
 template <typename I>
 __device__ __forceinline__ unsigned emb_key(I id, unsigned rows) {
@@ -63,8 +56,10 @@ __device__ __forceinline__ unsigned emb_key(I id, unsigned rows) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// forward: (1 << ls) lanes per token
+// forward: (1 << ls) lanes per token, EMB_C pieces of the row per lane (blockIdx.y: the next ones).  One token per group of lanes: with
+// several, 65536 tokens of 2048 bf16 took 79 .. 87 us instead of 59 = 5.6 TB/s of its 332 MB, the rate of a large copy.
 // ---------------------------------------------------------------------------------------------
+#define EMB_C 4
 template <typename T, int V, typename I>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ table, long tstride, const I* __restrict__ ids,
                                                         T* __restrict__ out, long n, unsigned rows, int D, int ls, float scale) {
@@ -74,7 +69,8 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
   const unsigned key = emb_key(ids[t], rows);
   const bool live = key < rows;
   const T* row = table + (live ? (long)key * tstride : 0);
-  for (int p = lane * V; p < D; p += V << ls) {
+  const int p0 = (int)blockIdx.y * EMB_C * (V << ls), p1 = min(D, p0 + EMB_C * (V << ls));
+  for (int p = p0 + lane * V; p < p1; p += V << ls) {
     const int c = min(p, D - V);
     float f[V];
 #pragma unroll
@@ -315,9 +311,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I* __restrict_
 // A pass in ONE launch, for lists that a workgroup can read whole: every workgroup counts the digits of the whole list and of what
 // lies before its tile by itself (n / 1024 loads per thread from the L2) instead of waiting for two launches that do it once.
 #define ONE_WAVES (TILE / 64)
-#ifndef ONE_COPIES
 #define ONE_COPIES 2
-#endif
 template <typename I>
 __global__ __launch_bounds__(TILE) void embed_pass_kernel(const I* __restrict__ ids, const unsigned* __restrict__ keys_in,
                                                           const int* __restrict__ order_in, int n, unsigned rows, int shift, int bits,
@@ -922,7 +916,7 @@ static EmbPlan emb_plan(long n, long rows, int cols, int vec) {
   p.ranked = n <= RANK_MAX;
   int need = 1;
   while (need < 32 && ((unsigned long)rows >> need) != 0) need++;         // keys 0 .. rows
-  p.passes = p.ranked ? 0 : (need + 9) / 10;
+  p.passes = p.ranked ? 0 : (need + MAX_BITS - 1) / MAX_BITS;
   p.bits = p.ranked ? 0 : (need + p.passes - 1) / p.passes;
   p.tiles = (int)((n + TILE - 1) / TILE);
   const long lanes = n * (((cols + vec - 1) / vec + (1 << p.ls) - 1) >> p.ls << p.ls);       // lanes at one place per group
@@ -947,8 +941,8 @@ static EmbPlan emb_plan(long n, long rows, int cols, int vec) {
     p.keys[i] = take(i == 0 || p.passes > 1 ? 4 * (size_t)n : 0);
     p.order[i] = take(i == 0 || p.passes > 1 ? 4 * (size_t)n : 0);
   }
-  p.hist = take(p.ranked ? 0 : (size_t)p.tiles * (4u << p.bits));
-  p.total = take(p.ranked ? 0 : 4u << p.bits);
+  p.hist = take(n <= ONE_MAX ? 0 : (size_t)p.tiles * (4u << p.bits));
+  p.total = take(n <= ONE_MAX ? 0 : 4u << p.bits);
   p.part = take(p.shares > 1 ? (size_t)p.shares * 2 * cols * 4 : 0);
   p.bytes = at;
   return p;
@@ -980,7 +974,8 @@ template <typename T, int V, typename I>
 static void emb_forward(const void* table, long tstride, const void* ids, void* out, long n, long rows, int cols, float scale,
                         hipStream_t s) {
   const int ls = row_lanes_log2(cols, V);
-  hipLaunchKernelGGL((embed_fwd_kernel<T, V, I>), dim3((unsigned)((n + (256 >> ls) - 1) / (256 >> ls))), dim3(256), 0, s,
+  const int wide = EMB_C * (V << ls);
+  hipLaunchKernelGGL((embed_fwd_kernel<T, V, I>), dim3((unsigned)((n + (256 >> ls) - 1) / (256 >> ls)), (cols + wide - 1) / wide), dim3(256), 0, s,
                      (const T*)table, tstride, (const I*)ids, (T*)out, n, (unsigned)rows, cols, ls, scale);
 }
 
@@ -992,6 +987,8 @@ extern "C" int ns_embedding_forward(const void* table, long table_stride, const 
   NS_REQUIRE(ids && out && (table || rows == 0), "ns_embedding_forward: null pointer");
   NS_REQUIRE(n <= EMB_MAX_TOKENS && rows <= 0x7fffffffL && cols >= 1 && cols <= EMB_MAX_COLS && table_stride >= 0,
              "ns_embedding_forward: bad shape (n %ld <= 2^25, rows %ld < 2^31, cols %d in 1 .. %d)", n, rows, cols, EMB_MAX_COLS);
+  NS_REQUIRE(row_aligned(table, dtype) && row_aligned(out, dtype) && (uintptr_t)ids % (ids_are_64 ? 8 : 4) == 0,
+             "ns_embedding_forward: a pointer is not aligned to its elements");
   hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto t) {
     using T = decltype(t);
@@ -1096,6 +1093,8 @@ extern "C" int ns_embedding_backward(const void* dout, long dout_stride, int dty
   NS_REQUIRE(grad && (n == 0 || (dout && ids)) && (ws || p.bytes == 0), "ns_embedding_backward: null pointer");
   NS_REQUIRE(ws_bytes >= p.bytes, "ns_embedding_backward: workspace of %zu bytes, %zu needed", ws_bytes, p.bytes);
   NS_REQUIRE(((uintptr_t)ws % 16) == 0, "ns_embedding_backward: the workspace needs 16-byte alignment");
+  NS_REQUIRE(row_aligned(dout, dtype) && row_aligned(grad, grad_dtype) && (uintptr_t)ids % (ids_are_64 ? 8 : 4) == 0,
+             "ns_embedding_backward: a pointer is not aligned to its elements");
   hipStream_t s = (hipStream_t)stream;
   const unsigned* keys = nullptr;
   const int* order = nullptr;

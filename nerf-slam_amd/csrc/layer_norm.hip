@@ -8,6 +8,8 @@
 // its output: LPR lanes hold NV pieces of 16 bytes each.  The backward pass keeps the two weight gradients of its lanes' columns in f32
 // registers over all the rows that a workgroup takes, so they cost one partial row pair per workgroup and a second, small launch that
 // adds those in a fixed order: no atomics, the same bits on every run.  All sums are f32; every output is rounded once.
+// Measured (copies of this size run at 5.0 .. 5.4 TB/s): forward 16384 x 4096 bf16 51 us = 5.3 TB/s, 230400 x 128 f16 19 us = 6.2 (half of
+// it stays in the caches); backward 81 us = 5.0 TB/s and 37 us = 4.8.
 #include "rows.h"
 
 #define LN_MAX_COLS 16384
@@ -93,9 +95,9 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T
         q += f[j][i] * f[j][i];
       }
     row_sum2<LPR>(s, q, red[1]);
-    const float m2 = s * inv_d, var = fmaxf(q * inv_d - m2 * m2, 0.0f), rs = 1.0f / sqrtf(var + eps);
+    const float m2 = s * inv_d, v0 = q * inv_d - m2 * m2, var = v0 < 0.0f ? 0.0f : v0, rs = 1.0f / sqrtf(var + eps);   // (a NaN stays)
     if (lane == 0 && mean) {
-      mean[r] = m1 + m2;
+      mean[r] = m2 == m2 ? m1 + m2 : m1;                        // (an infinity in the row: the mean is one, m2 is a NaN)
       rstd[r] = rs;
     }
 #pragma unroll
@@ -239,7 +241,7 @@ __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __r
 // Calls f(LPR, NV) with the lanes per row and pieces per lane of a row of D elements.  Up to 128 pieces a wave (or less) holds a row
 // and no barrier is needed; beyond, four waves; beyond 1024 pieces, sixteen.  Of the shapes for 513 .. 1024 pieces the forward pass takes
 // four waves with four pieces per lane, the backward pass, whose sums need the registers, eight waves with two
-// (8192 x 8192 bf16: forward 51 against 56 us, backward 132 against 88).
+// (8192 x 8192 bf16: forward 51 against 56 us, backward 132 against 80).
 template <int N>
 struct LnInt { static constexpr int v = N; };
 
@@ -270,26 +272,25 @@ static bool ln_types(int dtype, int wdtype, F f) {
   return true;
 }
 
-// workgroups: enough to fill the chip, few enough that the weights' registers are filled, and (backward) a partial row pair left, once
-// per many rows
-#ifndef LN_F256
-#define LN_F64 8192
-#define LN_F256 4096
-#define LN_F2564 1024
-#define LN_F1024 256
-#endif
-#ifndef LN_B256
-#define LN_B64 768
-#define LN_B256 1024
-#define LN_B2562 512
-#define LN_B512 256
-#define LN_B1024 256
-#endif
+// Workgroups by shape: enough to fill the chip, few enough that weights are fetched (and, backward, a partial row pair is left) once per
+// many rows.  Measured neighbours, us: forward 512 columns bf16 (8192) 23.7, half / twice as many 25.2 / 26.4; 4096 columns (4096) 50.7,
+// half / twice 55.3 / 54.4; 8192 columns (1024) 51, 512 / 4096 72 / 65; 16384 columns (256) 64, 1024 69.  Backward 128 columns f16
+// (768) 38.8, 512 / 2048 39.8 / 44.9; 771 columns f32 (1024) 67, 768 / 2048 77 / 75; 4096 columns (512) 81, 256 / 768 86 / 86; 8192
+// columns (256) 80, 512 87; 16384 columns (256) 97, 512 107.
+#define LN_FWD_WAVE 8192      // up to a wave per row
+#define LN_FWD_256 4096       // four waves, one or two pieces per lane
+#define LN_FWD_256_4 1024     // four waves, four pieces
+#define LN_FWD_1024 256
+#define LN_BWD_WAVE 768
+#define LN_BWD_256_1 1024
+#define LN_BWD_256_2 512
+#define LN_BWD_512 256
+#define LN_BWD_1024 256
 static int ln_blocks(long n, int D, int vec, bool back) {
   const int pieces = (D + vec - 1) / vec;
   const int per = pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 128 ? 4 : 1;
-  const int most = pieces <= 128 ? (back ? LN_B64 : LN_F64) : pieces <= 256 ? (back ? LN_B256 : LN_F256)
-                   : pieces <= 512 ? (back ? LN_B2562 : LN_F256) : pieces <= 1024 ? (back ? LN_B512 : LN_F2564) : (back ? LN_B1024 : LN_F1024);
+  const int most = pieces <= 128 ? (back ? LN_BWD_WAVE : LN_FWD_WAVE) : pieces <= 256 ? (back ? LN_BWD_256_1 : LN_FWD_256)
+                   : pieces <= 512 ? (back ? LN_BWD_256_2 : LN_FWD_256) : pieces <= 1024 ? (back ? LN_BWD_512 : LN_FWD_256_4) : (back ? LN_BWD_1024 : LN_FWD_1024);
   const long want = (n + per - 1) / per;
   return (int)(want < most ? want : most);
 }
@@ -302,6 +303,9 @@ extern "C" int ns_layer_norm_forward(const void* x, long x_stride, const void* w
   NS_REQUIRE((mean == nullptr) == (rstd == nullptr), "ns_layer_norm_forward: mean and rstd come together");
   if (n == 0) return NS_OK;
   NS_REQUIRE(x && y, "ns_layer_norm_forward: null pointer");
+  NS_REQUIRE(row_aligned(x, dtype) && row_aligned(y, dtype) && row_aligned(weight, wdtype) && row_aligned(bias, wdtype) &&
+                 row_aligned(mean, NS_F32) && row_aligned(rstd, NS_F32),
+             "ns_layer_norm_forward: a pointer is not aligned to its elements");
   const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
@@ -333,6 +337,10 @@ extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void
              "ns_layer_norm_backward: weight, dweight and dbias come together");
   const size_t need = weight ? ns_layer_norm_backward_workspace_bytes(n, cols, dtype) : 0;
   NS_REQUIRE(ws_bytes >= need && (ws || need == 0), "ns_layer_norm_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  NS_REQUIRE(row_aligned(dy, dtype) && row_aligned(x, dtype) && row_aligned(dx, dtype) && row_aligned(weight, wdtype) &&
+                 row_aligned(dweight, wdtype) && row_aligned(dbias, wdtype) && row_aligned(mean, NS_F32) && row_aligned(rstd, NS_F32) &&
+                 row_aligned(ws, NS_F32),
+             "ns_layer_norm_backward: a pointer is not aligned to its elements");
   const int blocks = ln_blocks(n, cols, dtype == NS_F32 ? 4 : 8, true);
   const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
     using T = decltype(t);

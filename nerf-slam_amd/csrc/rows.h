@@ -80,6 +80,8 @@ __device__ __forceinline__ void row_pin(RowPiece<T, N>& v) {
   __builtin_memcpy(&v, &q, sizeof(q));
 }
 
+static inline bool row_aligned(const void* p, int dtype) { return (uintptr_t)p % (dtype == NS_F32 ? 4 : 2) == 0; }
+
 // lanes that share a row: the power of two that covers its 16-byte pieces, at least 1, at most 64
 static inline int row_lanes_log2(int D, int vec) {
   const int pieces = (D + vec - 1) / vec;

@@ -74,7 +74,7 @@ def lookup64(table, ids, scale):
 @pytest.mark.parametrize("n,v,d,kind,idt", [
     (1, 1, 1, "even", torch.int32), (1, 100, 64, "even", torch.int64), (3, 5, 7, "pad", torch.int64), (257, 31, 8, "skew", torch.int32),
     (1000, 50, 33, "pad", torch.int32), (100, 7, 771, "even", torch.int64), (65, 300, 1024, "pad", torch.int64),
-    (4099, 1000, 32, "sorted", torch.int32), (5, 2, 65536, "even", torch.int32), (17, 3, 5, "none", torch.int64)])
+    (4099, 1000, 32, "sorted", torch.int32), (5, 2, 65536, "even", torch.int32), (1, 3, 5000, "even", torch.int64), (40, 9, 8200, "pad", torch.int64), (17, 3, 5, "none", torch.int64)])
 def test_embedding(dev, n, v, d, kind, idt, dtype):
     g = gen(dev, n + d)
     table, ids = randn(g, v, d, dtype=dtype), make_ids(g, n, v, kind, idt)
@@ -126,7 +126,8 @@ SIZES = [(1, 1, 1), (1, 40, 16), (15, 3, 5), (16, 3, 8), (17, 3, 8), (33, 1000, 
          (5000, 7, 12), (6001, 900, 771),
          (8192, 300, 8), (8193, 300, 8), (8193, 1023, 4), (9000, 1024, 12), (20000, 70000, 3), (40000, 5, 16), (4097, 5000, 2050),
          (8200, 512, 33), (9300, 512, 64), (30000, 64, 3), (12345, 1, 31), (10240, 513, 32), (9100, 1023, 20), (9200, 1024, 20),
-         (32768, 60000, 6), (32769, 60000, 6), (16385, 65535, 8), (16384, 65536, 8), (8195, 4000000, 9)]
+         (32768, 60000, 6), (32769, 60000, 6), (16385, 65535, 8), (16384, 65536, 8), (8195, 4000000, 9),
+         (300, 400000, 3), (1, 300000, 4), (4096, 300000, 9)]
 
 
 @pytest.mark.parametrize("kind", ["even", "skew", "pad"])
@@ -277,12 +278,13 @@ def test_layer_norm_keeps_the_spread_of_rows_far_from_zero(dev):
 
 def test_layer_norm_bad_values_stay_in_their_row(dev):
     g = gen(dev, 4)
+    keep = [i for i in range(12) if i not in (3, 7)]
     for d in (24, 128, 777, 3000):
         x = randn(g, 12, d, dtype=BF16)
         clean = rows.layer_norm(x)
         x[3, d - 1], x[7, 0] = float("nan"), float("inf")
-        y = rows.layer_norm(x)
-        keep = [i for i in range(12) if i not in (3, 7)]
+        y, mean, rstd = rows.layer_norm(x, stats=True)
+        assert mean[3].isnan() and mean[7] == float("inf") and rstd[3].isnan() and rstd[7].isnan() and mean[keep].isfinite().all() and rstd[keep].isfinite().all()
         assert torch.equal(y[keep], clean[keep]) and y[3].isnan().all() and y[7].isnan().all()
     const = rows.layer_norm(torch.full((4, 100), 3.0, device=dev), stats=True)       # no spread at all
     assert not const[0].any() and torch.allclose(const[2], torch.full((4,), 1e-5, device=dev).rsqrt(), rtol=1e-6)

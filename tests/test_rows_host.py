@@ -88,7 +88,13 @@ def test_abi_refusals():
     _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, P, 1, L(3), L((1 << 26) + 1), 257, C.c_float(1), P, big, None), "2^27")
     assert f.ns_embedding_backward(None, L(4), 1, None, 0, None, 1, L(3), L(0), 4, C.c_float(1), None, z, None) == 0
 
+    odd = C.c_void_p(4097)
+    _refused(f.ns_embedding_forward(odd, L(4), P, 0, P, 1, L(3), L(5), 4, C.c_float(1), None), "aligned")
+    _refused(f.ns_embedding_forward(P, L(4), C.c_void_p(4100), 1, P, 1, L(3), L(5), 4, C.c_float(1), None), "aligned")
+    _refused(f.ns_embedding_backward(P, L(4), 1, P, 0, C.c_void_p(4098), 2, L(3), L(5), 4, C.c_float(1), P, big, None), "aligned")
     e = C.c_float(1e-5)
+    _refused(f.ns_layer_norm_forward(odd, L(4), None, None, 2, P, None, None, 2, L(3), 4, e, None), "aligned")
+    _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, C.c_void_p(4098), P, 2, P, P, P, 2, L(3), 4, P, big, None), "aligned")
     _refused(f.ns_layer_norm_forward(None, L(4), None, None, 2, P, None, None, 2, L(3), 4, e, None), "null pointer")
     _refused(f.ns_layer_norm_forward(P, L(4), None, None, 2, P, P, None, 2, L(3), 4, e, None), "together")
     _refused(f.ns_layer_norm_forward(P, L(4), P, P, 1, P, P, P, 2, L(3), 4, e, None), "weight dtype")
