@@ -11,15 +11,14 @@
 //   few rows     up to FEW_ROWS rows of up to 16 lanes: two launches; a workgroup sorts and sums a tile of tokens, then the tiles' sums are
 //                added per row (embed_tile_kernel, embed_rows_kernel; 262144 tokens of 32 f16, 512 rows: 14 us, 28 in the next form)
 //   general      sort, sums over equal shares of the sorted list -- so that a row that a tenth of the tokens name costs no more than any
-//                other --, join (16384 tokens of 1024 bf16, 50000 rows: 45 us = 3.0 TB/s of its 135 MB)
+//                other --, join (16384 tokens of 1024 bf16, 50000 rows: 40 us = 3.4 TB/s of its 135 MB)
 //     sort   n <= RANK_MAX: one launch, a token's place counted directly (embed_rank_kernel); longer: radix passes of up to 10 bits, one
 //            launch each up to ONE_MAX tokens (embed_pass_kernel), beyond as histogram, prefix, scatter
 //     sums   a group of lanes walks consecutive places and sums runs of equal ids in f32 registers (emb_sum_share); a run inside the
-//            workgroup's share is final, one that crosses its ends leaves one f32 partial row per share (embed_sum_kernel, which also
-//            writes the rows without tokens)
+//            workgroup's share is final, one that crosses its ends leaves one f32 partial row per share (embed_sum_kernel)
 //     join   the share in which a crossing run begins adds its partial rows in order (embed_join_kernel)
-// The general form moves little more than dout and the gradient; beside them it is bound by the latency of its four or five launches,
-// each a chain of dependent loads (sort 20 us, sums 22, join 4 of the 45).
+// The general form moves little more than dout and the gradient; beside them it is bound by the latency of its launches, each a chain of
+// dependent loads (sort 24 us with the gradient's zeros written beside it, sums 11, join 4 of the 40).
 //
 // Columns: a lane holds V of them, 16 bytes, or one where a row is shorter than 16 bytes.  The last piece of a row ends with the row, so
 // where D is no multiple of V it overlaps the one before: both lanes form the same sums in the same order and store the same bits.
@@ -48,7 +47,6 @@
 #define SUM_U 8              // rows that a lane has on their way; 16: 78 instead of 61 us at 65536 tokens of 512 (fewer waves fit), 4: equal
 #define GROUP 8              // places of the sorted list per group of lanes, doubled (up to 128) while more than GROUP_WAVES waves are
 #define GROUP_WAVES 2048     // at work.  4096 / 8192 waves: 55 / 54 instead of 49 us at 16384 tokens of 1024
-#define ZERO_ROWS 8          // table rows per wave that looks for rows without tokens; 32: 15.4 instead of 13.6 us at 3001 tokens, equal elsewhere
 
 template <typename I>
 __device__ __forceinline__ unsigned emb_key(I id, unsigned rows) {
@@ -85,6 +83,30 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
 }
 
 // ---------------------------------------------------------------------------------------------
+// Rows without tokens: every launch of the sort, a few workgroups bound by latency, also writes a part of the whole gradient with zeros
+// (workgroups from `sort` on); the sums that follow write the rows that have tokens again.
+// ---------------------------------------------------------------------------------------------
+#define FILL_BYTES (1 << 14)     // per workgroup, up to FILL_BLOCKS of them: more stores in flight hold up the sort's loads
+#define FILL_BLOCKS 128          // (16384 tokens of 1024 bf16, 50000 rows: 40 us; 240: 41, 512: 44; with the zeros written by the sums: 46)
+struct EmbFill {
+  char* at;
+  long bytes;      // of whole elements
+  int sort;        // workgroups that sort
+};
+
+__device__ __forceinline__ void emb_fill(const EmbFill& f, int threads) {
+  typedef int v4i __attribute__((ext_vector_type(4), aligned(2)));
+  const long step = (long)((int)gridDim.x - f.sort) * threads * 16;
+  for (long o = ((long)((int)blockIdx.x - f.sort) * threads + threadIdx.x) * 16; o < f.bytes; o += step) {
+    if (o + 16 <= f.bytes) {
+      __builtin_nontemporal_store(v4i{0, 0, 0, 0}, reinterpret_cast<v4i*>(f.at + o));
+    } else {
+      for (long i = o; i < f.bytes; i += 2) *reinterpret_cast<short*>(f.at + i) = 0;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
 // sort, short lists: the place of token t is the number of tokens with a smaller key, or the same key and a smaller index: n^2 compares
 // at two vector instructions.  A workgroup places RANK_TOKENS tokens; its 16 waves, and the parts of a wave, each compare them with their
 // part of the list, which lies in LDS.
@@ -93,7 +115,8 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
 #define RANK_TOKENS 16       // = RANK_WAVES: wave w compares the workgroup's tokens with its w-th
 template <typename I>
 __global__ __launch_bounds__(64 * RANK_WAVES) void embed_rank_kernel(const I* __restrict__ ids, int n, unsigned rows,
-                                                                     unsigned* __restrict__ keys, int* __restrict__ order) {
+                                                                     unsigned* __restrict__ keys, int* __restrict__ order, EmbFill fill) {
+  if ((int)blockIdx.x >= fill.sort) return emb_fill(fill, 64 * RANK_WAVES);
   constexpr int THREADS = 64 * RANK_WAVES, PARTS = THREADS / RANK_TOKENS;
   __shared__ __align__(16) unsigned k[RANK_MAX];
   __shared__ int cnt[RANK_WAVES][64];
@@ -155,7 +178,8 @@ __device__ __forceinline__ unsigned emb_key_at(const I* __restrict__ ids, const 
 template <typename I>
 __global__ __launch_bounds__(256) void embed_hist_kernel(const I* __restrict__ ids, const unsigned* __restrict__ keys_in, long n,
                                                          unsigned rows, int shift, int bins, int used,
-                                                         int* __restrict__ hist) {
+                                                         int* __restrict__ hist, EmbFill fill) {
+  if ((int)blockIdx.x >= fill.sort) return emb_fill(fill, 256);
   __shared__ int h[COPIES * MAX_BINS];
   const int tid = threadIdx.x, copy = tid & (COPIES - 1);
   for (int i = tid; i < COPIES * bins; i += 256) h[i] = 0;
@@ -178,7 +202,9 @@ __global__ __launch_bounds__(256) void embed_hist_kernel(const I* __restrict__ i
 
 // hist[tile][digit] -> tokens of that digit in earlier tiles; total[digit].  64 digits per workgroup (one per lane), the tiles shared by
 // its 16 waves, 16 loads in flight each.
-__global__ __launch_bounds__(1024) void embed_prefix_kernel(int* __restrict__ hist, int tiles, int bins, int* __restrict__ total) {
+__global__ __launch_bounds__(1024) void embed_prefix_kernel(int* __restrict__ hist, int tiles, int bins, int* __restrict__ total,
+                                                            EmbFill fill) {
+  if ((int)blockIdx.x >= fill.sort) return emb_fill(fill, 1024);
   __shared__ int sums[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int d = blockIdx.x * 64 + lane;
@@ -226,8 +252,9 @@ template <typename I>
 __global__ __launch_bounds__(256) void embed_scatter_kernel(const I* __restrict__ ids, const unsigned* __restrict__ keys_in,
                                                             const int* __restrict__ order_in, long n, unsigned rows, int shift,
                                                             int bits, int used, const int* __restrict__ hist,
-                                                            const int* __restrict__ total,
-                                                            unsigned* __restrict__ keys_out, int* __restrict__ order_out) {
+                                                            const int* __restrict__ total, unsigned* __restrict__ keys_out,
+                                                            int* __restrict__ order_out, EmbFill fill) {
+  if ((int)blockIdx.x >= fill.sort) return emb_fill(fill, 256);
   __shared__ int off[4][MAX_BINS];
   __shared__ int part[4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -315,7 +342,8 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const I* __restrict_
 template <typename I>
 __global__ __launch_bounds__(TILE) void embed_pass_kernel(const I* __restrict__ ids, const unsigned* __restrict__ keys_in,
                                                           const int* __restrict__ order_in, int n, unsigned rows, int shift, int bits,
-                                                          unsigned* __restrict__ keys_out, int* __restrict__ order_out) {
+                                                          unsigned* __restrict__ keys_out, int* __restrict__ order_out, EmbFill fill) {
+  if ((int)blockIdx.x >= fill.sort) return emb_fill(fill, TILE);
   extern __shared__ int lds[];       // [bins][ONE_COPIES] before the tile, [bins][ONE_COPIES] from it on, [waves][bins] 16 bit of each wave
   __shared__ int part[ONE_WAVES];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, copy = tid & (ONE_COPIES - 1);
@@ -385,17 +413,8 @@ __global__ __launch_bounds__(TILE) void embed_pass_kernel(const I* __restrict__ 
 // ---------------------------------------------------------------------------------------------
 // sums over the sorted list
 // ---------------------------------------------------------------------------------------------
-// first place in [lo, hi) whose key is not below `key`, for one lane
-__device__ __forceinline__ int emb_lower_bound(const unsigned* __restrict__ keys, int lo, int hi, unsigned key) {
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (keys[mid] < key) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// the same for a whole wave (uniform arguments): 64 probes a step, so three dependent loads where the other takes eighteen
+// first place in [lo, hi) whose key is not below `key`, for a wave (uniform arguments): 64 probes a step, so three dependent loads where
+// halving takes eighteen
 __device__ __forceinline__ int emb_lower_bound_wave(const unsigned* __restrict__ keys, int lo, int hi, unsigned key) {
   const int lane = threadIdx.x & 63;
   while (lo < hi) {
@@ -535,44 +554,18 @@ __device__ __forceinline__ void emb_sum_share(const T* __restrict__ from, long d
   }
 }
 
-// grid: (shares, then workgroups that write the rows without tokens) x pieces of the columns, the pieces of one share next to each
-// other, so that the rows of dout are read whole at about the same time.  A share is what a workgroup sums: `group`
+// grid: shares x pieces of the columns, the pieces of one share next to each other, so that the rows of dout are read whole at about the
+// same time.  A share is what a workgroup sums: `group`
 // places per group of lanes, (256 >> ls) groups.  The groups sum their runs in registers and meet in LDS, so that only the run that
 // enters the share and the one that leaves it become partial rows: part [shares][2][D], row 0 entered, row 1 begins here and leaves.
 template <typename T, int V, typename G>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ dout, long dstride, const unsigned* __restrict__ keys,
                                                         const int* __restrict__ order, int n, unsigned rows, int D, int ls, int group,
-                                                        int shares, int pieces, float scale, G* __restrict__ grad,
+                                                        int pieces, float scale, G* __restrict__ grad,
                                                         float* __restrict__ part) {
   const int tid = threadIdx.x, block = (int)(blockIdx.x / (unsigned)pieces), lane = tid & ((1 << ls) - 1);
   const int first = (int)(blockIdx.x - (unsigned)block * pieces) * (V << ls) + lane * V, c = min(first, D - V);
   const bool col = first < D;
-  if (block >= shares) {                           // rows that no token names
-    const int wl = tid & 63;
-    const long r0 = ((long)(block - shares) * 4 + (tid >> 6)) * ZERO_ROWS;
-    if (r0 >= (long)rows) return;
-    const int lo = emb_lower_bound_wave(keys, 0, n, (unsigned)r0);
-    const unsigned next = lo + wl < n ? keys[lo + wl] : 0xffffffffu;
-    bool empty = false;
-    if (__ballot(next >= (unsigned)r0 + ZERO_ROWS)) {          // 64 places show all tokens of these rows
-#pragma unroll
-      for (int i = 0; i < ZERO_ROWS; i++) {
-        const bool none = __ballot(next == (unsigned)r0 + i) == 0;
-        if (wl == i) empty = none && r0 + i < (long)rows;
-      }
-    } else if (wl < ZERO_ROWS && r0 + wl < (long)rows) {
-      const unsigned r = (unsigned)(r0 + wl);
-      const int p = emb_lower_bound(keys, lo, n, r);
-      empty = p >= n || keys[p] != r;
-    }
-    const unsigned long long m = __ballot(empty);
-    float z[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) z[i] = 0.0f;
-    for (int i = wl >> ls; i < ZERO_ROWS; i += 64 >> ls)
-      if (col && ((m >> i) & 1)) row_put<G, V, true>(grad + (r0 + i) * D + c, z);
-    return;
-  }
   auto store = [&](unsigned r, float* acc) {
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] *= scale;
@@ -1011,12 +1004,25 @@ extern "C" size_t ns_embedding_backward_workspace_bytes(long n, long rows, int c
 }
 
 template <typename I>
-static void emb_sort(const EmbPlan& p, const I* ids, char* ws, int n, unsigned rows, const unsigned** keys, const int** order,
-                     hipStream_t s) {
+static void emb_sort(const EmbPlan& p, const I* ids, char* ws, int n, unsigned rows, void* grad, long grad_bytes, const unsigned** keys,
+                     const int** order, hipStream_t s) {
   unsigned* k[2] = {(unsigned*)(ws + p.keys[0]), (unsigned*)(ws + p.keys[1])};
   int* o[2] = {(int*)(ws + p.order[0]), (int*)(ws + p.order[1])};
+  // the gradient's zeros, in equal parts over the launches
+  const int launches = p.ranked ? 1 : n <= ONE_MAX ? p.passes : 3 * p.passes;
+  const long part = ((grad_bytes + launches - 1) / launches + 15) / 16 * 16;
+  long filled = 0;
+  EmbFill fill;
+  auto grid = [&](int sort) {                                  // workgroups of a launch that sorts with `sort` of them; sets `fill`
+    fill.at = (char*)grad + filled;
+    fill.bytes = grad_bytes - filled < part ? grad_bytes - filled : part;
+    fill.sort = sort;
+    filled += fill.bytes;
+    return dim3((unsigned)(sort + min((fill.bytes + FILL_BYTES - 1) / FILL_BYTES, (long)FILL_BLOCKS)));
+  };
   if (p.ranked) {
-    hipLaunchKernelGGL(embed_rank_kernel<I>, dim3((n + RANK_TOKENS - 1) / RANK_TOKENS), dim3(64 * RANK_WAVES), 0, s, ids, n, rows, k[0], o[0]);
+    const dim3 g = grid((n + RANK_TOKENS - 1) / RANK_TOKENS);
+    hipLaunchKernelGGL(embed_rank_kernel<I>, g, dim3(64 * RANK_WAVES), 0, s, ids, n, rows, k[0], o[0], fill);
     *keys = k[0];
     *order = o[0];
     return;
@@ -1027,18 +1033,21 @@ static void emb_sort(const EmbPlan& p, const I* ids, char* ws, int n, unsigned r
   const unsigned* ki = nullptr;
   const int* oi = nullptr;
   for (int i = 0; i < p.passes; i++) {
+    const int shift = i * p.bits;
     if (n <= ONE_MAX) {
-      hipLaunchKernelGGL(embed_pass_kernel<I>, dim3(p.tiles), dim3(TILE), (2 * ONE_COPIES + ONE_WAVES / 2) * sizeof(int) << p.bits, s, ids, ki, oi, n, rows,
-                         i * p.bits, p.bits, k[i & 1], o[i & 1]);
-      ki = k[i & 1];
-      oi = o[i & 1];
-      continue;
+      const dim3 g = grid(p.tiles);
+      hipLaunchKernelGGL(embed_pass_kernel<I>, g, dim3(TILE), (2 * ONE_COPIES + ONE_WAVES / 2) * sizeof(int) << p.bits, s, ids, ki, oi, n,
+                         rows, shift, p.bits, k[i & 1], o[i & 1], fill);
+    } else {
+      const int used = (int)min((unsigned)bins, (rows >> shift) + 1);        // digits that occur: the keys end at `rows`
+      dim3 g = grid(p.tiles);
+      hipLaunchKernelGGL(embed_hist_kernel<I>, g, dim3(256), 0, s, ids, ki, (long)n, rows, shift, bins, used, hist, fill);
+      g = grid((used + 63) / 64);
+      hipLaunchKernelGGL(embed_prefix_kernel, g, dim3(1024), 0, s, hist, p.tiles, used, total, fill);
+      g = grid(p.tiles);
+      hipLaunchKernelGGL(embed_scatter_kernel<I>, g, dim3(256), 0, s, ids, ki, oi, (long)n, rows, shift, p.bits, used, hist, total, k[i & 1],
+                         o[i & 1], fill);
     }
-    const int used = (int)min((unsigned)bins, (rows >> (i * p.bits)) + 1);      // digits that occur: the keys end at `rows`
-    hipLaunchKernelGGL(embed_hist_kernel<I>, dim3(p.tiles), dim3(256), 0, s, ids, ki, (long)n, rows, i * p.bits, bins, used, hist);
-    hipLaunchKernelGGL(embed_prefix_kernel, dim3((used + 63) / 64), dim3(1024), 0, s, hist, p.tiles, used, total);
-    hipLaunchKernelGGL(embed_scatter_kernel<I>, dim3(p.tiles), dim3(256), 0, s, ids, ki, oi, (long)n, rows, i * p.bits, p.bits, used,
-                       hist, total, k[i & 1], o[i & 1]);
     ki = k[i & 1];
     oi = o[i & 1];
   }
@@ -1066,10 +1075,9 @@ static void emb_few(const EmbPlan& p, const T* dout, long dstride, const I* ids,
 template <typename T, int V, typename G>
 static void emb_sums(const EmbPlan& p, const T* dout, long dstride, const unsigned* keys, const int* order, int n, unsigned rows,
                      int cols, float scale, G* grad, float* part, hipStream_t s) {
-  const int zero_blocks = (int)(((long)rows + 4 * ZERO_ROWS - 1) / (4 * ZERO_ROWS));
   const int col_blocks = (cols + (V << p.ls) - 1) / (V << p.ls), share = p.group * (256 >> p.ls);
-  hipLaunchKernelGGL((embed_sum_kernel<T, V, G>), dim3((unsigned)(p.shares + zero_blocks) * col_blocks), dim3(256), 0, s, dout, dstride, keys,
-                     order, n, rows, cols, p.ls, p.group, p.shares, col_blocks, scale, grad, part);
+  hipLaunchKernelGGL((embed_sum_kernel<T, V, G>), dim3((unsigned)p.shares * col_blocks), dim3(256), 0, s, dout, dstride, keys, order, n, rows,
+                     cols, p.ls, p.group, col_blocks, scale, grad, part);
   if (p.shares > 1) {
     // one workgroup per share up to 1024 of them (in a skewed list most are the beginning of a crossing run, each a chain of loads);
     // beyond, a workgroup looks at up to 64
@@ -1099,8 +1107,9 @@ extern "C" int ns_embedding_backward(const void* dout, long dout_stride, int dty
   const unsigned* keys = nullptr;
   const int* order = nullptr;
   if (!p.small && !p.few) {
-    if (ids_are_64) emb_sort(p, (const int64_t*)ids, (char*)ws, (int)n, (unsigned)rows, &keys, &order, s);
-    else emb_sort(p, (const int32_t*)ids, (char*)ws, (int)n, (unsigned)rows, &keys, &order, s);
+    const long bytes = rows * cols * (grad_dtype == NS_F32 ? 4 : 2);
+    if (ids_are_64) emb_sort(p, (const int64_t*)ids, (char*)ws, (int)n, (unsigned)rows, grad, bytes, &keys, &order, s);
+    else emb_sort(p, (const int32_t*)ids, (char*)ws, (int)n, (unsigned)rows, grad, bytes, &keys, &order, s);
     NS_CHECK_LAUNCH("embedding_backward: sort");
   }
   auto go = [&](auto t) {
