@@ -115,19 +115,71 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T
 }
 
 // ---------------------------------------------------------------------------------------------
-// backward.  part: [workgroups][2][D] f32 (dw | db); a single workgroup writes dweight and dbias itself (no weight: nobody).
+// backward.  part: [workgroups][2][D] f32 (dw | db), or nullptr: no weight.
+//
+// FEW: few rows, one launch, no part.  The weight gradients are formed by further workgroups (from row_blocks on), ln_columns pieces of the
+// columns each over all rows, which are read a second time (they lie in the caches): dw and db need no sum over a row, mean and rstd are given.
 // ---------------------------------------------------------------------------------------------
-template <typename T, typename W, int LPR, int NV>
+template <int BLOCK>
+constexpr int ln_columns() { return BLOCK / 64; }    // 64 lanes share a piece's rows
+
+template <typename T, typename W, int BLOCK>
+__device__ __forceinline__ void layer_norm_columns(const T* __restrict__ dy, long dstride, const T* __restrict__ x, long xstride,
+                                                   const float* __restrict__ mean, const float* __restrict__ rstd, W* __restrict__ dweight,
+                                                   W* __restrict__ dbias, int n, int D, int block, float* __restrict__ red) {
+  constexpr int V = row_vec<T>(), COLUMNS = ln_columns<BLOCK>(), SUBS = BLOCK / COLUMNS, WAVES = BLOCK / 64;
+  const int piece = threadIdx.x % COLUMNS, c = (block * COLUMNS + piece) * V, wave = threadIdx.x / 64;
+  float sum[2][V];                                               // dw | db
+#pragma unroll
+  for (int i = 0; i < V; i++) sum[0][i] = sum[1][i] = 0.0f;
+  if (c < D) {
+#pragma unroll 4
+    for (int r = threadIdx.x / COLUMNS; r < n; r += SUBS) {
+      const RowPiece<T, V> p = row_load<T, V>(x + (long)r * xstride, c, D), d = row_load<T, V>(dy + (long)r * dstride, c, D);
+      const float mu = mean[r], rs = rstd[r];
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const float u = (float)d.e[i];
+        sum[0][i] += u * (((float)p.e[i] - mu) * rs);
+        sum[1][i] += u;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+#pragma unroll
+      for (int o = 32; o >= COLUMNS; o >>= 1) sum[k][i] += __shfl_down(sum[k][i], o, 64);
+      if (threadIdx.x % 64 < COLUMNS) red[((wave * 2 + k) * COLUMNS + piece) * V + i] = sum[k][i];
+    }
+  __syncthreads();
+  if (threadIdx.x < 2 * COLUMNS) {
+    const int k = threadIdx.x / COLUMNS;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      acc[i] = 0.0f;
+#pragma unroll
+      for (int q = 0; q < WAVES; q++) acc[i] += red[((q * 2 + k) * COLUMNS + piece) * V + i];
+    }
+    if (c < D) row_store<W, V>(k ? dbias : dweight, c, D, acc);
+  }
+}
+
+template <typename T, typename W, int LPR, int NV, bool FEW>
 __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T* __restrict__ dy, long dstride, const T* __restrict__ x,
                                                                          long xstride, const float* __restrict__ mean,
                                                                          const float* __restrict__ rstd, const W* __restrict__ w,
                                                                          T* __restrict__ dx, float* __restrict__ part, W* __restrict__ dweight,
-                                                                         W* __restrict__ dbias, long n, int D, float inv_d) {
+                                                                         W* __restrict__ dbias, long n, int D, float inv_d, int row_blocks) {
   constexpr int V = row_vec<T>(), BLOCK = ln_block<LPR>(), ROWS = BLOCK / LPR;
   __shared__ float red[2][LPR > 64 ? LPR / 64 : 1][2];
-  __shared__ float cols[ROWS > 1 ? BLOCK * (V + 1) : 1];
+  __shared__ float cols[FEW ? BLOCK / 32 * ln_columns<BLOCK>() * V : ROWS > 1 ? BLOCK * (V + 1) : 1];
+  if (FEW && (int)blockIdx.x >= row_blocks)
+    return layer_norm_columns<T, W, BLOCK>(dy, dstride, x, xstride, mean, rstd, dweight, dbias, (int)n, D, (int)blockIdx.x - row_blocks, cols);
   const int lane = threadIdx.x % LPR;
-  const long step = (long)gridDim.x * ROWS;
+  const long step = (long)row_blocks * ROWS;
   RowPiece<W, V> wp[NV];
   float dw[NV][V], db[NV][V];
 #pragma unroll
@@ -168,8 +220,10 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
       for (int i = 0; i < V; i++) {
         const float u = (float)d[j].e[i];                       // (0 behind the end of the row, so g and both gradients are)
         const float h = ((float)p[j].e[i] - mu) * rs, g = w ? u * (float)wp[j].e[i] : u;
-        db[j][i] += u;
-        dw[j][i] += u * h;
+        if (!FEW) {
+          db[j][i] += u;
+          dw[j][i] += u * h;
+        }
         s += g;
         q += g * h;
       }
@@ -188,7 +242,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
       row_store<T, V>(dx + r * D, (j * LPR + lane) * V, D, f);
     }
   }
-  if (!w) return;
+  if (FEW || !part) return;
 #pragma unroll
   for (int k = 0; k < 2; k++)
 #pragma unroll
@@ -206,10 +260,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
             for (int i = 0; i < V; i++) acc[i] += cols[(t * LPR + lane) * (V + 1) + i];
         }
       }
-      if (threadIdx.x < LPR) {
-        if (gridDim.x == 1) row_store<W, V>(k ? dbias : dweight, (j * LPR + lane) * V, D, acc);
-        else row_store<float, V>(part + ((long)blockIdx.x * 2 + k) * D, (j * LPR + lane) * V, D, acc);
-      }
+      if (threadIdx.x < LPR) row_store<float, V>(part + ((long)blockIdx.x * 2 + k) * D, (j * LPR + lane) * V, D, acc);
     }
 }
 
@@ -286,6 +337,10 @@ static bool ln_types(int dtype, int wdtype, F f) {
 #define LN_BWD_256_2 512
 #define LN_BWD_512 256
 #define LN_BWD_1024 256
+// rows up to which the backward pass is one launch without a workspace (three allocations and a launch less: 14 us instead of 18 a call
+// where the host is what it waits for).  On the device, us, one launch | two: 16 rows of 771 bf16 4.5 | 7.7, 256: 6.5 | 8.7, 512: 8.7 | 8.4;
+// 512 rows of 128: 10.7 | 6.5, of 4096: 13.4 | 18.1; 1024 rows lose at every width
+#define LN_FEW_ROWS 512
 static int ln_blocks(long n, int D, int vec, bool back) {
   const int pieces = (D + vec - 1) / vec;
   const int per = pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 128 ? 4 : 1;
@@ -322,9 +377,8 @@ extern "C" int ns_layer_norm_forward(const void* x, long x_stride, const void* w
 }
 
 extern "C" size_t ns_layer_norm_backward_workspace_bytes(long n, int cols, int dtype) {
-  if (n <= 0 || cols < 1 || cols > LN_MAX_COLS) return 0;
-  const int blocks = ln_blocks(n, cols, dtype == NS_F32 ? 4 : 8, true);
-  return blocks > 1 ? (size_t)blocks * 2 * cols * 4 : 0;
+  if (n <= LN_FEW_ROWS || cols < 1 || cols > LN_MAX_COLS) return 0;
+  return (size_t)ln_blocks(n, cols, dtype == NS_F32 ? 4 : 8, true) * 2 * cols * 4;
 }
 
 extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void* x, long x_stride, const float* mean, const float* rstd,
@@ -345,14 +399,17 @@ extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void
   const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
-    if (n > 0)
+    const bool few = n <= LN_FEW_ROWS;
+    if (n > 0 || (weight && few))
       ln_shape<row_vec<T>(), true>(cols, [&](auto lpr, auto nv) {
-        constexpr int L = decltype(lpr)::v, N = decltype(nv)::v;
-        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, L, N>), dim3(blocks), dim3(ln_block<L>()), 0, (hipStream_t)stream, (const T*)dy,
-                           dy_stride, (const T*)x, x_stride, mean, rstd, (const W*)weight, (T*)dx, (float*)ws, (W*)dweight, (W*)dbias, n, cols,
-                           1.0f / (float)cols);
+        constexpr int L = decltype(lpr)::v, N = decltype(nv)::v, wide = ln_columns<ln_block<L>()>() * row_vec<T>();
+        const int extra = weight && few ? (cols + wide - 1) / wide : 0;
+        auto kernel = few ? layer_norm_bwd_kernel<T, W, L, N, true> : layer_norm_bwd_kernel<T, W, L, N, false>;
+        hipLaunchKernelGGL(kernel, dim3(blocks + extra), dim3(ln_block<L>()), 0, (hipStream_t)stream, (const T*)dy, dy_stride, (const T*)x,
+                           x_stride, mean, rstd, (const W*)weight, (T*)dx, weight ? (float*)ws : nullptr, (W*)dweight, (W*)dbias, n, cols,
+                           1.0f / (float)cols, blocks);
       });
-    if (weight && blocks != 1)                                 // (0 workgroups, no rows: zeros)
+    if (weight && !few)
       hipLaunchKernelGGL(layer_norm_wgrad_kernel<W>, dim3((2 * cols + 63) / 64), dim3(1024), 0, (hipStream_t)stream, (const float*)ws, blocks,
                          cols, (W*)dweight, (W*)dbias);
   });

@@ -323,7 +323,8 @@ def check_norm_backward(got, dout, x, mean, rstd, w, what):
 
 @pytest.mark.parametrize("d", COLS)
 def test_layer_norm_backward(dev, d):
-    for dtype, wdtype, n in ((F32, F32, 5), (F16, F32, 37), (F16, F16, 1), (BF16, BF16, 66), (BF16, F32, 3), (F32, None, 70)):
+    for dtype, wdtype, n in ((F32, F32, 5), (F16, F32, 37), (F16, F16, 1), (BF16, BF16, 66), (BF16, F32, 3), (F32, None, 70), (F32, F32, 512),
+                             (BF16, BF16, 511), (F16, F32, 513), (F16, None, 600), (F32, F32, 700)):
         g = gen(dev, d * 3 + n)
         x = (2.0 * randn(g, n, d) + 0.7 * randn(g, 1, d) - 1.0).to(dtype)
         dout = randn(g, n, d, dtype=dtype)
@@ -476,7 +477,7 @@ def test_nothing_is_written_outside_the_outputs(dev):
     g = gen(dev, 13)
     f = lib()
     L = C.c_long
-    for n, v, d in ((37, 11, 33), (9000, 700, 5), (70, 300, 520), (5000, 70, 33), (20000, 2000, 70)):
+    for n, v, d in ((37, 11, 33), (9000, 700, 5), (70, 300, 520), (5000, 70, 33), (20000, 2000, 70), (600, 5, 2000)):
         ids = make_ids(g, n, v, "pad", torch.int32)
         x = randn(g, n * d + 1, dtype=F16)[1:]                                  # 2-byte alignment
         table = randn(g, v * d + 1, dtype=F16)[1:]

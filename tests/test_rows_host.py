@@ -120,4 +120,4 @@ def test_workspace_sizes():
     for n in (8192, 8193, 1 << 20):
         assert emb(L(n), L(1000), 64, 2) >= 8 * n and emb(L(n), L(1000), 64, 3) % 16 == 0
     assert emb(L(1 << 25), L(1 << 19), 65536, 1) > 2 ** 31          # (no 32-bit arithmetic in it)
-    assert ln(L(1), 64, 2) == 0 and ln(L(1000), 64, 2) % 512 == 0 and ln(L(1 << 20), 64, 2) > 0
+    assert ln(L(512), 64, 2) == 0 and ln(L(1000), 64, 2) % 512 == 0 and ln(L(1 << 20), 64, 2) > 0
