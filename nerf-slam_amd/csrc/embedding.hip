@@ -350,22 +350,19 @@ __global__ __launch_bounds__(TILE) void embed_pass_kernel(const I* __restrict__ 
   const int bins = 1 << bits, t0 = (int)blockIdx.x * TILE;
   int* cnt = lds;
   unsigned short* off = reinterpret_cast<unsigned short*>(lds + 2 * ONE_COPIES * bins);    // (places below ONE_MAX)
-  for (int i = tid; i < (2 * ONE_COPIES + ONE_WAVES / 2) * bins; i += TILE) lds[i] = 0;
-  __syncthreads();
   const int t = t0 + tid;
   const bool in = t < n;
+  constexpr int U = ONE_MAX / TILE;
+  unsigned k[U];                                           // the whole list, loads first
+#pragma unroll
+  for (int u = 0; u < U; u++) k[u] = u * TILE < n ? emb_key_at(ids, keys_in, min(u * TILE + tid, n - 1), rows) : 0u;
   const unsigned key = emb_key_at(ids, keys_in, min(t, n - 1), rows);
   const int from = order_in ? order_in[min(t, n - 1)] : t;
-  constexpr int U = 16;                                    // loads in flight
-  for (int b = 0; b < n; b += U * TILE) {
-    unsigned k[U];
+  for (int i = tid; i < (2 * ONE_COPIES + ONE_WAVES / 2) * bins; i += TILE) lds[i] = 0;
+  __syncthreads();
 #pragma unroll
-    for (int u = 0; u < U; u++) k[u] = b + u * TILE < n ? emb_key_at(ids, keys_in, min(b + u * TILE + tid, n - 1), rows) : 0u;
-#pragma unroll
-    for (int u = 0; u < U; u++)
-      if (b + u * TILE + tid < n)
-        atomicAdd(&cnt[((b + u * TILE < t0 ? 0 : bins) + ((k[u] >> shift) & (bins - 1))) * ONE_COPIES + copy], 1);
-  }
+  for (int u = 0; u < U; u++)
+    if (u * TILE + tid < n) atomicAdd(&cnt[((u * TILE < t0 ? 0 : bins) + ((k[u] >> shift) & (bins - 1))) * ONE_COPIES + copy], 1);
   const int d = (key >> shift) & (bins - 1);
   const unsigned long long same = emb_same_digit(d, bits, in);
   const int before = __popcll(same & ((1ull << lane) - 1));
