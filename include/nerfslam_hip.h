@@ -753,8 +753,8 @@ int ns_embedding_forward(const void* table, long table_stride, const void* ids, 
 /* grad[r] = scale * sum of dout[t] over the tokens t with ids[t] == r; every row of grad [rows, cols] is written (0 without tokens),
  * rows of dout whose id lies outside [0, rows) are not used.  grad_dtype: dtype or NS_F32.  The tokens are sorted by id on the device
  * and the sums run over the sorted list in a fixed order: the same inputs give the same bits.  rows * ceil(cols / 256) <= 2^27.
- *   ws: ns_embedding_backward_workspace_bytes(n, rows, cols, dtype) bytes, 16-byte aligned, contents irrelevant; calls that may be in flight
- *   at the same time must not share it.                                                                                        */
+ *   ws: ns_embedding_backward_workspace_bytes(n, rows, cols, dtype) bytes (0 for short lists, at most about 4 per element of dout + 16
+ *   per token), 16-byte aligned, contents irrelevant; calls that may be in flight at the same time must not share it.          */
 size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols, int dtype);
 int ns_embedding_backward(const void* dout, long dout_stride, int dtype, const void* ids, int ids_are_64, void* grad, int grad_dtype,
                           long n, long rows, int cols, float scale, void* ws, size_t ws_bytes, void* stream);
@@ -765,7 +765,7 @@ int ns_layer_norm_forward(const void* x, long x_stride, const void* weight, cons
                           float* rstd, int dtype, long n, int cols, float eps, void* stream);
 /* With g = dy * weight and xh = (x - mean) * rstd:  dx = rstd * (g - mean(g) - xh * mean(g xh)), dweight = sum over rows of dy xh,
  * dbias = sum over rows of dy (both of wdtype, in a fixed order).  weight, dweight and dbias: all or none (none: dx alone).
- *   ws: ns_layer_norm_backward_workspace_bytes(n, cols, dtype) bytes (none without a weight), as above.                        */
+ *   ws: ns_layer_norm_backward_workspace_bytes(n, cols, dtype) bytes (none without a weight; 0 for few rows), as above.        */
 size_t ns_layer_norm_backward_workspace_bytes(long n, int cols, int dtype);
 int ns_layer_norm_backward(const void* dy, long dy_stride, const void* x, long x_stride, const float* mean, const float* rstd,
                            const void* weight, int wdtype, void* dx, void* dweight, void* dbias, int dtype, long n, int cols, void* ws,

@@ -737,6 +737,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const float* __restrict
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; i++) acc[i] = 0.0f;
+  bool some = false;
   constexpr int U = 8;
   for (int t = sub; t < tiles; t += U * subs) {
     unsigned word[U];
@@ -748,8 +749,10 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const float* __restrict
         const RowPiece<float, V> v = row_get<float, V>(from + (long)(t + u * subs) * D);
 #pragma unroll
         for (int i = 0; i < V; i++) acc[i] += v.e[i];
+        some = true;
       }
   }
+  const bool named = __syncthreads_or(some);                   // (a row without tokens is 0 whatever the scale)
 #pragma unroll
   for (int i = 0; i < V; i++) red[tid][i] = acc[i];
   for (int o = subs / 2; o > 0; o >>= 1) {
@@ -761,7 +764,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const float* __restrict
   }
   if (sub == 0 && first < D) {
 #pragma unroll
-    for (int i = 0; i < V; i++) acc[i] = red[tid][i] * scale;
+    for (int i = 0; i < V; i++) acc[i] = named ? red[tid][i] * scale : 0.0f;
     row_put<G, V, true>(grad + (long)row * D + c, acc);
   }
 }

@@ -127,7 +127,7 @@ SIZES = [(1, 1, 1), (1, 40, 16), (15, 3, 5), (16, 3, 8), (17, 3, 8), (33, 1000, 
          (8192, 300, 8), (8193, 300, 8), (8193, 1023, 4), (9000, 1024, 12), (20000, 70000, 3), (40000, 5, 16), (4097, 5000, 2050),
          (8200, 512, 33), (9300, 512, 64), (30000, 64, 3), (12345, 1, 31), (10240, 513, 32), (9100, 1023, 20), (9200, 1024, 20),
          (32768, 60000, 6), (32769, 60000, 6), (16385, 65535, 8), (16384, 65536, 8), (8195, 4000000, 9),
-         (300, 400000, 3), (1, 300000, 4), (4096, 300000, 9)]
+         (20, 600, 9000), (5, 3, 65536), (9000, 30, 3000), (300, 400000, 3), (1, 300000, 4), (4096, 300000, 9)]
 
 
 @pytest.mark.parametrize("kind", ["even", "skew", "pad"])
@@ -186,6 +186,13 @@ def test_embedding_backward_strides_padding_and_empty(dev):
     assert torch.equal(rows.embedding_backward(wide.view(5, 100, 96), ids.view(5, 100), 40), rows.embedding_backward(wide, ids, 40))
     assert not rows.embedding_backward(wide[:0], ids[:0], 40).any()
     assert rows.embedding_backward(wide, ids, 0).shape == (0, 96)
+
+
+@pytest.mark.parametrize("n,v,d", [(50, 300, 8), (9000, 300, 8), (9000, 3000, 8), (40000, 3000, 8)])
+def test_embedding_backward_rows_without_tokens_are_zero_whatever_the_scale(dev, n, v, d):
+    ids = torch.arange(n, device=dev) % (v // 2) * 2            # the even rows
+    got = rows.embedding_backward(torch.ones((n, d), device=dev), ids, v, scale=float("inf"))
+    assert not got[1::2].any() and (got[ids.unique()] == float("inf")).all()
 
 
 def test_embedding_gradient_is_the_difference_of_the_lookup(dev):
