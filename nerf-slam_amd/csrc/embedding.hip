@@ -729,7 +729,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void embed_tile_kernel(const T* __r
 template <typename G, int V>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const float* __restrict__ part, const unsigned* __restrict__ touched, int tiles,
                                                          int D, int ls, float scale, G* __restrict__ grad) {
-  __shared__ float red[256][V + 1];
+  __shared__ float red[4][1 << FEW_LANES][V + 1];
+  __shared__ bool named[4];
   const int tid = threadIdx.x, sub = tid >> ls, subs = 256 >> ls;
   const int row = blockIdx.x;
   const int first = (tid & ((1 << ls) - 1)) * V, c = min(first, D - V);
@@ -752,19 +753,22 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const float* __restrict
         some = true;
       }
   }
-  const bool named = __syncthreads_or(some);                   // (a row without tokens is 0 whatever the scale)
+  // the sub-groups of a wave meet through shuffles, the waves through LDS; a row without tokens is 0 whatever the scale
+  const int wide = 1 << ls, w = tid >> 6, lane = tid & 63;
+  for (int o = wide; o < 64; o <<= 1)
 #pragma unroll
-  for (int i = 0; i < V; i++) red[tid][i] = acc[i];
-  for (int o = subs / 2; o > 0; o >>= 1) {
-    __syncthreads();
-    if (sub < o) {
+    for (int i = 0; i < V; i++) acc[i] += __shfl_xor(acc[i], o, 64);
+  if (lane < wide) {
 #pragma unroll
-      for (int i = 0; i < V; i++) red[tid][i] += red[tid + (o << ls)][i];
-    }
+    for (int i = 0; i < V; i++) red[w][lane][i] = acc[i];
   }
-  if (sub == 0 && first < D) {
+  const bool any = __ballot(some) != 0;
+  if (lane == 0) named[w] = any;
+  __syncthreads();
+  if (tid < wide && first < D) {
+    const bool all = named[0] | named[1] | named[2] | named[3];
 #pragma unroll
-    for (int i = 0; i < V; i++) acc[i] = named ? red[tid][i] * scale : 0.0f;
+    for (int i = 0; i < V; i++) acc[i] = all ? (red[0][tid][i] + red[1][tid][i] + red[2][tid][i] + red[3][tid][i]) * scale : 0.0f;
     row_put<G, V, true>(grad + (long)row * D + c, acc);
   }
 }
