@@ -8,8 +8,8 @@
 // its output: LPR lanes hold NV pieces of 16 bytes each.  The backward pass keeps the two weight gradients of its lanes' columns in f32
 // registers over all the rows that a workgroup takes, so they cost one partial row pair per workgroup and a second, small launch that
 // adds those in a fixed order: no atomics, the same bits on every run.  All sums are f32; every output is rounded once.
-// Measured (copies of this size run at 5.0 .. 5.4 TB/s): forward 16384 x 4096 bf16 51 us = 5.3 TB/s, 230400 x 128 f16 19 us = 6.2 (half of
-// it stays in the caches); backward 81 us = 5.0 TB/s and 37 us = 4.8.
+// Measured (copies of this size run at 5.0 .. 5.4 TB/s): forward 16384 x 4096 bf16 46 us = 5.8 TB/s (parts of it stay in the caches), 230400 x
+// 128 f16 20 us = 6.0; backward 81 us = 5.0 TB/s and 36 us = 4.9.
 #include "rows.h"
 
 #define LN_MAX_COLS 16384
@@ -48,40 +48,51 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2]) {
   }
 }
 
+// columns [c, c + V) of a piece and how many of them the piece before it owns: the last piece of a row ends with the row and overlaps its
+// neighbour where D is no multiple of V.  Both lanes form and store the same bits there; a row's sums leave the first `skip` out.  skip >= V:
+// no piece (its lane reads the last one).  Pieces cut off element by element cost more (32768 x 1500 bf16: forward 53 instead of 38 us, backward 106 instead of 63).
+// whole: known not to be the last.
+template <int V>
+__device__ __forceinline__ void ln_piece(int piece, int D, int& c, int& skip, bool whole = false) {
+  c = whole ? piece * V : min(piece * V, D - V);
+  skip = whole ? 0 : piece * V - c;
+}
+
 template <int LPR>
-constexpr int ln_block() { return LPR > 256 ? LPR : 256; }
+constexpr int ln_block() { return LPR > 64 ? LPR : 256; }
 
 // ---------------------------------------------------------------------------------------------
 // forward.  Two sums over the row, in turn: the mean, then sum d and sum d^2 of the deviations d = x - mean.  The first of these is what
 // rounding left of the mean; taking it out again keeps the deviations exact where |mean| is far above the row's spread.
 // ---------------------------------------------------------------------------------------------
-template <typename T, typename W, int LPR, int NV>
+template <typename T, typename W, int V, int LPR, int NV>
 __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T* __restrict__ x, long xstride, const W* __restrict__ w,
                                                                          const W* __restrict__ b, T* __restrict__ y,
                                                                          float* __restrict__ mean, float* __restrict__ rstd, long n, int D,
                                                                          float inv_d, float eps) {
-  constexpr int V = row_vec<T>(), ROWS = ln_block<LPR>() / LPR;
+  constexpr int ROWS = ln_block<LPR>() / LPR;
   __shared__ float red[2][LPR > 64 ? LPR / 64 : 1][2];   // (per sum: the other sum's barrier lies between two uses)
   const int lane = threadIdx.x % LPR;
   const long step = (long)gridDim.x * ROWS;
   RowPiece<W, V> wp[NV], bp[NV];
+  int c[NV], skip[NV];
 #pragma unroll
   for (int j = 0; j < NV; j++) {
-    const int c = (j * LPR + lane) * V;
-    if (w) wp[j] = row_load<W, V>(w, c, D);
-    if (b) bp[j] = row_load<W, V>(b, c, D);
+    ln_piece<V>(j * LPR + lane, D, c[j], skip[j], j < NV / 2);
+    if (w) wp[j] = row_get<W, V>(w + c[j]);
+    if (b) bp[j] = row_get<W, V>(b + c[j]);
   }
-  for (long r = (long)blockIdx.x * ROWS + threadIdx.x / LPR; r < n; r += step) {
+  for (long r = (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / LPR : 0); r < n; r += step) {
     RowPiece<T, V> p[NV];
 #pragma unroll
-    for (int j = 0; j < NV; j++) p[j] = row_load<T, V>(x + r * xstride, (j * LPR + lane) * V, D);
+    for (int j = 0; j < NV; j++) p[j] = row_get<T, V>(x + r * xstride + c[j]);
     float f[NV][V], s = 0.0f, q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
       for (int i = 0; i < V; i++) {
         f[j][i] = (float)p[j].e[i];
-        s += f[j][i];
+        s += i >= skip[j] ? f[j][i] : 0.0f;
       }
     row_sum2<LPR>(s, q, red[0]);
     const float m1 = s * inv_d;
@@ -90,9 +101,10 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T
     for (int j = 0; j < NV; j++)
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        f[j][i] = (j * LPR + lane) * V + i < D ? f[j][i] - m1 : 0.0f;
-        s += f[j][i];
-        q += f[j][i] * f[j][i];
+        f[j][i] -= m1;
+        const float d = i >= skip[j] ? f[j][i] : 0.0f;
+        s += d;
+        q += d * d;
       }
     row_sum2<LPR>(s, q, red[1]);
     const float m2 = s * inv_d, v0 = q * inv_d - m2 * m2, var = v0 < 0.0f ? 0.0f : v0, rs = 1.0f / sqrtf(var + eps);   // (a NaN stays)
@@ -109,7 +121,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T
         if (b) v += (float)bp[j].e[i];
         f[j][i] = v;
       }
-      row_store<T, V>(y + r * D, (j * LPR + lane) * V, D, f[j]);
+      if (skip[j] < V) row_put<T, V, false>(y + r * D + c[j], f[j]);
     }
   }
 }
@@ -123,19 +135,21 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T
 template <int BLOCK>
 constexpr int ln_columns() { return BLOCK / 64; }    // 64 lanes share a piece's rows
 
-template <typename T, typename W, int BLOCK>
+template <typename T, typename W, int V, int BLOCK>
 __device__ __forceinline__ void layer_norm_columns(const T* __restrict__ dy, long dstride, const T* __restrict__ x, long xstride,
                                                    const float* __restrict__ mean, const float* __restrict__ rstd, W* __restrict__ dweight,
                                                    W* __restrict__ dbias, int n, int D, int block, float* __restrict__ red) {
-  constexpr int V = row_vec<T>(), COLUMNS = ln_columns<BLOCK>(), SUBS = BLOCK / COLUMNS, WAVES = BLOCK / 64;
-  const int piece = threadIdx.x % COLUMNS, c = (block * COLUMNS + piece) * V, wave = threadIdx.x / 64;
+  constexpr int COLUMNS = ln_columns<BLOCK>(), SUBS = BLOCK / COLUMNS, WAVES = BLOCK / 64;
+  const int piece = threadIdx.x % COLUMNS, wave = threadIdx.x / 64;
+  int c, skip;
+  ln_piece<V>(block * COLUMNS + piece, D, c, skip);
   float sum[2][V];                                               // dw | db
 #pragma unroll
   for (int i = 0; i < V; i++) sum[0][i] = sum[1][i] = 0.0f;
-  if (c < D) {
+  if (skip < V) {
 #pragma unroll 4
     for (int r = threadIdx.x / COLUMNS; r < n; r += SUBS) {
-      const RowPiece<T, V> p = row_load<T, V>(x + (long)r * xstride, c, D), d = row_load<T, V>(dy + (long)r * dstride, c, D);
+      const RowPiece<T, V> p = row_get<T, V>(x + (long)r * xstride + c), d = row_get<T, V>(dy + (long)r * dstride + c);
       const float mu = mean[r], rs = rstd[r];
 #pragma unroll
       for (int i = 0; i < V; i++) {
@@ -163,47 +177,58 @@ __device__ __forceinline__ void layer_norm_columns(const T* __restrict__ dy, lon
 #pragma unroll
       for (int q = 0; q < WAVES; q++) acc[i] += red[((q * 2 + k) * COLUMNS + piece) * V + i];
     }
-    if (c < D) row_store<W, V>(k ? dbias : dweight, c, D, acc);
+    if (skip < V) row_put<W, V, false>((k ? dbias : dweight) + c, acc);
   }
 }
 
-template <typename T, typename W, int LPR, int NV, bool FEW>
+template <typename T, typename W, int V, int LPR, int NV, bool FEW>
 __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T* __restrict__ dy, long dstride, const T* __restrict__ x,
                                                                          long xstride, const float* __restrict__ mean,
                                                                          const float* __restrict__ rstd, const W* __restrict__ w,
                                                                          T* __restrict__ dx, float* __restrict__ part, W* __restrict__ dweight,
                                                                          W* __restrict__ dbias, long n, int D, float inv_d, int row_blocks) {
-  constexpr int V = row_vec<T>(), BLOCK = ln_block<LPR>(), ROWS = BLOCK / LPR;
+  constexpr int BLOCK = ln_block<LPR>(), ROWS = BLOCK / LPR;
   __shared__ float red[2][LPR > 64 ? LPR / 64 : 1][2];
   __shared__ float cols[FEW ? BLOCK / 32 * ln_columns<BLOCK>() * V : ROWS > 1 ? BLOCK * (V + 1) : 1];
   if (FEW && (int)blockIdx.x >= row_blocks)
-    return layer_norm_columns<T, W, BLOCK>(dy, dstride, x, xstride, mean, rstd, dweight, dbias, (int)n, D, (int)blockIdx.x - row_blocks, cols);
+    return layer_norm_columns<T, W, V, BLOCK>(dy, dstride, x, xstride, mean, rstd, dweight, dbias, (int)n, D, (int)blockIdx.x - row_blocks, cols);
   const int lane = threadIdx.x % LPR;
   const long step = (long)row_blocks * ROWS;
+  // 128 registers at sixteen waves: the widest f32 rows have none left to keep where their pieces lie
+  int c[NV], skip[NV];
+  constexpr bool TIGHT = LPR == 1024 && NV == 4;
+  auto places = [&]() {
+    int end = D;
+    asm volatile("" : "+s"(end));                               // (formed anew)
+#pragma unroll
+    for (int j = 0; j < NV; j++) ln_piece<V>(j * LPR + lane, end, c[j], skip[j], j < NV / 2);
+  };
   RowPiece<W, V> wp[NV];
   float dw[NV][V], db[NV][V];
 #pragma unroll
   for (int j = 0; j < NV; j++) {
-    if (w) wp[j] = row_load<W, V>(w, (j * LPR + lane) * V, D);
+    ln_piece<V>(j * LPR + lane, D, c[j], skip[j], j < NV / 2);
+    if (w) wp[j] = row_get<W, V>(w + c[j]);
 #pragma unroll
     for (int i = 0; i < V; i++) dw[j][i] = db[j][i] = 0.0f;
   }
   // the next row is on its way while this one is worked on, where the registers allow it
-    constexpr bool AHEAD = LPR < 1024;
+  constexpr bool AHEAD = LPR < 1024;
   RowPiece<T, V> pn[NV], dn[NV];
   float mun = 0.0f, rsn = 0.0f;
   auto fetch = [&](long r) {
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      pn[j] = row_load<T, V>(x + r * xstride, (j * LPR + lane) * V, D);
-      dn[j] = row_load<T, V>(dy + r * dstride, (j * LPR + lane) * V, D);
+      pn[j] = row_get<T, V>(x + r * xstride + c[j]);
+      dn[j] = row_get<T, V>(dy + r * dstride + c[j]);
     }
     mun = mean[r];
     rsn = rstd[r];
   };
-  long r = (long)blockIdx.x * ROWS + threadIdx.x / LPR;
+  long r = (long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / LPR : 0);
   if (AHEAD && r < n) fetch(r);
   for (int turn = 0; r < n; r += step, turn ^= 1) {
+    if (TIGHT) places();
     if (!AHEAD) fetch(r);
     RowPiece<T, V> p[NV], d[NV];
 #pragma unroll
@@ -215,20 +240,21 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
     if (AHEAD && r + step < n) fetch(r + step);
     float s = 0.0f, q = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+    for (int j = 0; j < NV; j++) {
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float u = (float)d[j].e[i];                       // (0 behind the end of the row, so g and both gradients are)
-        const float h = ((float)p[j].e[i] - mu) * rs, g = w ? u * (float)wp[j].e[i] : u;
+        const float u = (float)d[j].e[i], h = ((float)p[j].e[i] - mu) * rs, g = w ? u * (float)wp[j].e[i] : u;
         if (!FEW) {
           db[j][i] += u;
           dw[j][i] += u * h;
         }
-        s += g;
-        q += g * h;
+        s += i >= skip[j] ? g : 0.0f;
+        q += i >= skip[j] ? g * h : 0.0f;
       }
+    }
     row_sum2<LPR>(s, q, red[turn]);
     const float a = s * inv_d, b = q * inv_d;
+    if (TIGHT) places();
 #pragma unroll
     for (int j = 0; j < NV; j++) {
       row_pin(p[j]);                                            // g and xh are formed again from the 16-byte pieces: held over the sums
@@ -239,7 +265,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
         const float u = (float)d[j].e[i], h = ((float)p[j].e[i] - mu) * rs, g = w ? u * (float)wp[j].e[i] : u;
         f[i] = (g - a - h * b) * rs;
       }
-      row_store<T, V>(dx + r * D, (j * LPR + lane) * V, D, f);
+      if (skip[j] < V) row_put<T, V, false>(dx + r * D + c[j], f);
     }
   }
   if (FEW || !part) return;
@@ -260,7 +286,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
             for (int i = 0; i < V; i++) acc[i] += cols[(t * LPR + lane) * (V + 1) + i];
         }
       }
-      if (threadIdx.x < LPR) row_store<float, V>(part + ((long)blockIdx.x * 2 + k) * D, (j * LPR + lane) * V, D, acc);
+      if (threadIdx.x < LPR && skip[j] < V) row_put<float, V, false>(part + ((long)blockIdx.x * 2 + k) * D + c[j], acc);
     }
 }
 
@@ -294,22 +320,25 @@ __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __r
 // ---------------------------------------------------------------------------------------------
 // C ABI
 // ---------------------------------------------------------------------------------------------
-// Calls f(LPR, NV) with the lanes per row and pieces per lane of a row of D elements.  Up to 128 pieces a wave (or less) holds a row
-// and no barrier is needed; beyond, four waves; beyond 1024 pieces, sixteen.  Of the shapes for 513 .. 1024 pieces the forward pass takes
-// four waves with four pieces per lane, the backward pass, whose sums need the registers, eight waves with two
-// (8192 x 8192 bf16: forward 51 against 56 us, backward 132 against 80).
+// Calls f(V, LPR, NV) with the elements of a piece, the lanes per row and the pieces per lane of a row of D elements.  V is 16 bytes, or one
+// element where a row is shorter.  Up to 128 pieces a wave (or less) holds a row and no barrier is needed; beyond, 2 to 16 waves.  The
+// forward pass takes more pieces per lane, the backward pass, whose sums need the registers, more waves: 129 .. 256 pieces as 128 lanes of
+// two, forward 45 us (32768 x 2048 bf16; 256 of one: 47.5), backward 91 against 81; 513 .. 1024 as 256 of four, forward 51 (8192 x 8192; 512 of
+// two: 56), backward 132 against 80.  NV > 1 implies more than LPR * NV / 2 pieces: the first half of a lane's are whole.
 template <int N>
 struct LnInt { static constexpr int v = N; };
 
 template <int V, bool BACK, typename F>
-static void ln_shape(int D, F f) {
+static void ln_shape(int D, F g) {
   const int pieces = (D + V - 1) / V;
-  if (pieces <= 8) f(LnInt<8>(), LnInt<1>());
+  auto f = [&](auto lpr, auto nv) { g(LnInt<V>(), lpr, nv); };
+  if (D < V) g(LnInt<1>(), LnInt<8>(), LnInt<1>());
+  else if (pieces <= 8) f(LnInt<8>(), LnInt<1>());
   else if (pieces <= 16) f(LnInt<16>(), LnInt<1>());
   else if (pieces <= 32) f(LnInt<32>(), LnInt<1>());
   else if (pieces <= 64) f(LnInt<64>(), LnInt<1>());
   else if (pieces <= 128) f(LnInt<64>(), LnInt<2>());
-  else if (pieces <= 256) f(LnInt<256>(), LnInt<1>());
+  else if (pieces <= 256) f(LnInt<(BACK ? 256 : 128)>(), LnInt<(BACK ? 1 : 2)>());
   else if (pieces <= 512) f(LnInt<256>(), LnInt<2>());
   else if (pieces <= 1024) f(LnInt<(BACK ? 512 : 256)>(), LnInt<(BACK ? 2 : 4)>());
     else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
@@ -329,11 +358,12 @@ static bool ln_types(int dtype, int wdtype, F f) {
 }
 
 // Workgroups by shape: enough to fill the chip, few enough that weights are fetched (and, backward, a partial row pair is left) once per
-// many rows.  Measured neighbours, us: forward 512 columns bf16 (8192) 23.7, half / twice as many 25.2 / 26.4; 4096 columns (4096) 50.7,
-// half / twice 55.3 / 54.4; 8192 columns (1024) 51, 512 / 4096 72 / 65; 16384 columns (256) 64, 1024 69.  Backward 128 columns f16
+// many rows.  Measured neighbours, us: forward 512 columns bf16 (8192) 23.7, half / twice as many 25.2 / 26.4; 1500 columns (8192) 38.3,
+// half / twice 42.5 / 39.8; 4096 columns (4096) 50.7, half / twice 55.3 / 54.4; 8192 columns (1024) 51, 512 / 4096 72 / 65; 16384 columns (256) 64, 1024 69.  Backward 128 columns f16
 // (768) 38.8, 512 / 2048 39.8 / 44.9; 771 columns f32 (1024) 67, 768 / 2048 77 / 75; 4096 columns (512) 81, 256 / 768 86 / 86; 8192
 // columns (256) 80, 512 87; 16384 columns (256) 97, 512 107.
 #define LN_FWD_WAVE 8192      // up to a wave per row
+#define LN_FWD_128 8192       // two waves, two pieces
 #define LN_FWD_256 4096       // four waves, one or two pieces per lane
 #define LN_FWD_256_4 1024     // four waves, four pieces
 #define LN_FWD_1024 256
@@ -349,7 +379,7 @@ static bool ln_types(int dtype, int wdtype, F f) {
 static int ln_blocks(long n, int D, int vec, bool back) {
   const int pieces = (D + vec - 1) / vec;
   const int per = pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 128 ? 4 : 1;
-  const int most = pieces <= 128 ? (back ? LN_BWD_WAVE : LN_FWD_WAVE) : pieces <= 256 ? (back ? LN_BWD_256_1 : LN_FWD_256)
+  const int most = pieces <= 128 ? (back ? LN_BWD_WAVE : LN_FWD_WAVE) : pieces <= 256 ? (back ? LN_BWD_256_1 : LN_FWD_128)
                    : pieces <= 512 ? (back ? LN_BWD_256_2 : LN_FWD_256) : pieces <= 1024 ? (back ? LN_BWD_512 : LN_FWD_256_4) : (back ? LN_BWD_1024 : LN_FWD_1024);
   const long want = (n + per - 1) / per;
   return (int)(want < most ? want : most);
@@ -369,9 +399,9 @@ extern "C" int ns_layer_norm_forward(const void* x, long x_stride, const void* w
   const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
-    ln_shape<row_vec<T>(), false>(cols, [&](auto lpr, auto nv) {
-      constexpr int L = decltype(lpr)::v, N = decltype(nv)::v;
-      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, L, N>), dim3(ln_blocks(n, cols, row_vec<T>(), false)), dim3(ln_block<L>()), 0,
+    ln_shape<row_vec<T>(), false>(cols, [&](auto vec, auto lpr, auto nv) {
+      constexpr int V = decltype(vec)::v, L = decltype(lpr)::v, N = decltype(nv)::v;
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, V, L, N>), dim3(ln_blocks(n, cols, row_vec<T>(), false)), dim3(ln_block<L>()), 0,
                          (hipStream_t)stream, (const T*)x, x_stride, (const W*)weight, (const W*)bias, (T*)y, mean, rstd, n, cols,
                          1.0f / (float)cols, eps);
     });
@@ -406,10 +436,10 @@ extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void
     using W = decltype(u);
     const bool few = n <= LN_FEW_ROWS;
     if (n > 0 || (weight && few))
-      ln_shape<row_vec<T>(), true>(cols, [&](auto lpr, auto nv) {
-        constexpr int L = decltype(lpr)::v, N = decltype(nv)::v, wide = ln_columns<ln_block<L>()>() * row_vec<T>();
+      ln_shape<row_vec<T>(), true>(cols, [&](auto vec, auto lpr, auto nv) {
+        constexpr int V = decltype(vec)::v, L = decltype(lpr)::v, N = decltype(nv)::v, wide = ln_columns<ln_block<L>()>() * V;
         const int extra = weight && few ? (cols + wide - 1) / wide : 0;
-        auto kernel = few ? layer_norm_bwd_kernel<T, W, L, N, true> : layer_norm_bwd_kernel<T, W, L, N, false>;
+        auto kernel = few ? layer_norm_bwd_kernel<T, W, V, L, N, true> : layer_norm_bwd_kernel<T, W, V, L, N, false>;
         hipLaunchKernelGGL(kernel, dim3(blocks + extra), dim3(ln_block<L>()), 0, (hipStream_t)stream, (const T*)dy, dy_stride, (const T*)x,
                            x_stride, mean, rstd, (const W*)weight, (T*)dx, weight ? (float*)ws : nullptr, (W*)dweight, (W*)dbias, n, cols,
                            1.0f / (float)cols, blocks);

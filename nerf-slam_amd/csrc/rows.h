@@ -17,33 +17,6 @@ struct RowPiece {
 };
 
 template <typename T, int N>
-__device__ __forceinline__ RowPiece<T, N> row_load(const T* __restrict__ row, int c, int D) {
-  RowPiece<T, N> v;
-  if (c + N <= D) {
-    __builtin_memcpy(&v, row + c, sizeof(v));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) v.e[i] = c + i < D ? row[c + i] : (T)0.0f;
-  }
-  return v;
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void row_store(T* __restrict__ row, int c, int D, const float* f) {
-  RowPiece<T, N> v;
-#pragma unroll
-  for (int i = 0; i < N; i++) v.e[i] = (T)f[i];      // one rounding, to nearest even
-  if (c + N <= D) {
-    __builtin_memcpy(row + c, &v, sizeof(v));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++)
-      if (c + i < D) row[c + i] = v.e[i];
-  }
-}
-
-// whole pieces
-template <typename T, int N>
 __device__ __forceinline__ RowPiece<T, N> row_get(const T* __restrict__ at) {
   RowPiece<T, N> v;
   __builtin_memcpy(&v, at, sizeof(v));
@@ -73,11 +46,12 @@ __device__ __forceinline__ void row_put(T* __restrict__ at, const float* f) {
 template <typename T, int N>
 __device__ __forceinline__ void row_pin(RowPiece<T, N>& v) {
   typedef int v4i __attribute__((ext_vector_type(4)));
-  static_assert(sizeof(v) == sizeof(v4i), "a 16-byte piece");
-  v4i q;
-  __builtin_memcpy(&q, &v, sizeof(q));
-  asm volatile("" : "+v"(q));
-  __builtin_memcpy(&v, &q, sizeof(q));
+  if constexpr (sizeof(v) == sizeof(v4i)) {
+    v4i q;
+    __builtin_memcpy(&q, &v, sizeof(q));
+    asm volatile("" : "+v"(q));
+    __builtin_memcpy(&v, &q, sizeof(q));
+  }
 }
 
 static inline bool row_aligned(const void* p, int dtype) { return (uintptr_t)p % (dtype == NS_F32 ? 4 : 2) == 0; }
