@@ -133,7 +133,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T
 // columns each over all rows, which are read a second time (they lie in the caches): dw and db need no sum over a row, mean and rstd are given.
 // ---------------------------------------------------------------------------------------------
 template <int BLOCK>
-constexpr int ln_columns() { return BLOCK / 64; }    // 64 lanes share a piece's rows
+constexpr int ln_columns() { return BLOCK > 256 ? BLOCK / 64 : 4; }    // 32 or 64 lanes share a piece's rows
 
 template <typename T, typename W, int V, int BLOCK>
 __device__ __forceinline__ void layer_norm_columns(const T* __restrict__ dy, long dstride, const T* __restrict__ x, long xstride,
@@ -321,14 +321,13 @@ __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __r
 // C ABI
 // ---------------------------------------------------------------------------------------------
 // Calls f(V, LPR, NV) with the elements of a piece, the lanes per row and the pieces per lane of a row of D elements.  V is 16 bytes, or one
-// element where a row is shorter.  Up to 128 pieces a wave (or less) holds a row and no barrier is needed; beyond, 2 to 16 waves.  The
-// forward pass takes more pieces per lane, the backward pass, whose sums need the registers, more waves: 129 .. 256 pieces as 128 lanes of
-// two, forward 45 us (32768 x 2048 bf16; 256 of one: 47.5), backward 91 against 81; 513 .. 1024 as 256 of four, forward 51 (8192 x 8192; 512 of
-// two: 56), backward 132 against 80.  NV > 1 implies more than LPR * NV / 2 pieces: the first half of a lane's are whole.
+// element where a row is shorter.  Up to 128 pieces a wave (or less) holds a row and no barrier is needed; beyond, 2 to 16 waves.  Two
+// pieces per lane: 256 lanes of one piece take 47 us instead of 38 forward (32768 x 1500 bf16; backward the same 63), 256 lanes of four 55
+// instead of 52 and 82 instead of 80 (8192 x 8192).  NV > 1 implies more than LPR * NV / 2 pieces: the first half of a lane's are whole.
 template <int N>
 struct LnInt { static constexpr int v = N; };
 
-template <int V, bool BACK, typename F>
+template <int V, typename F>
 static void ln_shape(int D, F g) {
   const int pieces = (D + V - 1) / V;
   auto f = [&](auto lpr, auto nv) { g(LnInt<V>(), lpr, nv); };
@@ -338,9 +337,9 @@ static void ln_shape(int D, F g) {
   else if (pieces <= 32) f(LnInt<32>(), LnInt<1>());
   else if (pieces <= 64) f(LnInt<64>(), LnInt<1>());
   else if (pieces <= 128) f(LnInt<64>(), LnInt<2>());
-  else if (pieces <= 256) f(LnInt<(BACK ? 256 : 128)>(), LnInt<(BACK ? 1 : 2)>());
+  else if (pieces <= 256) f(LnInt<128>(), LnInt<2>());
   else if (pieces <= 512) f(LnInt<256>(), LnInt<2>());
-  else if (pieces <= 1024) f(LnInt<(BACK ? 512 : 256)>(), LnInt<(BACK ? 2 : 4)>());
+  else if (pieces <= 1024) f(LnInt<512>(), LnInt<2>());
     else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
   else if constexpr (V == 4) f(LnInt<1024>(), LnInt<4>());
 }
@@ -357,30 +356,29 @@ static bool ln_types(int dtype, int wdtype, F f) {
   return true;
 }
 
-// Workgroups by shape: enough to fill the chip, few enough that weights are fetched (and, backward, a partial row pair is left) once per
-// many rows.  Measured neighbours, us: forward 512 columns bf16 (8192) 23.7, half / twice as many 25.2 / 26.4; 1500 columns (8192) 38.3,
-// half / twice 42.5 / 39.8; 4096 columns (4096) 50.7, half / twice 55.3 / 54.4; 8192 columns (1024) 51, 512 / 4096 72 / 65; 16384 columns (256) 64, 1024 69.  Backward 128 columns f16
-// (768) 38.8, 512 / 2048 39.8 / 44.9; 771 columns f32 (1024) 67, 768 / 2048 77 / 75; 4096 columns (512) 81, 256 / 768 86 / 86; 8192
-// columns (256) 80, 512 87; 16384 columns (256) 97, 512 107.
-#define LN_FWD_WAVE 8192      // up to a wave per row
-#define LN_FWD_128 8192       // two waves, two pieces
-#define LN_FWD_256 4096       // four waves, one or two pieces per lane
-#define LN_FWD_256_4 1024     // four waves, four pieces
-#define LN_FWD_1024 256
-#define LN_BWD_WAVE 768
-#define LN_BWD_256_1 1024
-#define LN_BWD_256_2 512
-#define LN_BWD_512 256
-#define LN_BWD_1024 256
-// rows up to which the backward pass is one launch without a workspace (three allocations and a launch less: 14 us instead of 18 a call
-// where the host is what it waits for).  On the device, us, one launch | two: 16 rows of 771 bf16 4.5 | 7.7, 256: 6.5 | 8.7, 512: 8.7 | 8.4;
-// 512 rows of 128: 10.7 | 6.5, of 4096: 13.4 | 18.1; 1024 rows lose at every width
+// Most workgroups by shape: enough to fill the chip, few enough that weights are fetched (and, backward, a partial row pair is left) once per
+// many rows.  Measured neighbours, us.  Forward: 512 columns bf16 (8192) 24.6, half / twice as many 24.3 / 26.6; 1500 (8192) 38.5, 39.0 /
+// 39.5; 4096 (4096) 47, 51 / 47; 16384 (256) 57, twice / four times 59 / 64.  Backward: 128 f16 (768) 36.4, 512 / 1024 37.9 / 36.4; 1500
+// bf16 (1024) 63, 768 / 1536 68 / 80; 4096 (512) 82, 256 / 768 100 / 87; 8192 (256) 80, 512 / 768 87 / 92; 16384 (256) 90, 512 / 768 101 / 116.
+struct LnMost {
+  int forward, backward;
+};
+static LnMost ln_most(int pieces) {
+  if (pieces <= 128) return {8192, 768};      // up to a wave per row
+  if (pieces <= 256) return {8192, 1024};
+  if (pieces <= 512) return {4096, 512};
+  if (pieces <= 1024) return {1024, 256};
+  return {256, 256};
+}
+
+// rows up to which the backward pass is one launch without a workspace (an allocation and a launch less: 14 us instead of 18 a call where the
+// host is what it waits for).  On the device, us, one launch | two: 512 rows of 128 bf16 5.8 | 6.3, of 771: 6.3 | 7.0, of 4096: 9.6 | 16.8;
+// 1024 rows: 7.6 | 6.4, 11.8 | 8.3, 14.3 | 18.5
 #define LN_FEW_ROWS 512
 static int ln_blocks(long n, int D, int vec, bool back) {
   const int pieces = (D + vec - 1) / vec;
   const int per = pieces <= 8 ? 32 : pieces <= 16 ? 16 : pieces <= 32 ? 8 : pieces <= 128 ? 4 : 1;
-  const int most = pieces <= 128 ? (back ? LN_BWD_WAVE : LN_FWD_WAVE) : pieces <= 256 ? (back ? LN_BWD_256_1 : LN_FWD_128)
-                   : pieces <= 512 ? (back ? LN_BWD_256_2 : LN_FWD_256) : pieces <= 1024 ? (back ? LN_BWD_512 : LN_FWD_256_4) : (back ? LN_BWD_1024 : LN_FWD_1024);
+  const int most = back ? ln_most(pieces).backward : ln_most(pieces).forward;
   const long want = (n + per - 1) / per;
   return (int)(want < most ? want : most);
 }
@@ -399,7 +397,7 @@ extern "C" int ns_layer_norm_forward(const void* x, long x_stride, const void* w
   const bool ok = ln_types(dtype, wdtype, [&](auto t, auto u) {
     using T = decltype(t);
     using W = decltype(u);
-    ln_shape<row_vec<T>(), false>(cols, [&](auto vec, auto lpr, auto nv) {
+    ln_shape<row_vec<T>()>(cols, [&](auto vec, auto lpr, auto nv) {
       constexpr int V = decltype(vec)::v, L = decltype(lpr)::v, N = decltype(nv)::v;
       hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, V, L, N>), dim3(ln_blocks(n, cols, row_vec<T>(), false)), dim3(ln_block<L>()), 0,
                          (hipStream_t)stream, (const T*)x, x_stride, (const W*)weight, (const W*)bias, (T*)y, mean, rstd, n, cols,
@@ -436,7 +434,7 @@ extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void
     using W = decltype(u);
     const bool few = n <= LN_FEW_ROWS;
     if (n > 0 || (weight && few))
-      ln_shape<row_vec<T>(), true>(cols, [&](auto vec, auto lpr, auto nv) {
+      ln_shape<row_vec<T>()>(cols, [&](auto vec, auto lpr, auto nv) {
         constexpr int V = decltype(vec)::v, L = decltype(lpr)::v, N = decltype(nv)::v, wide = ln_columns<ln_block<L>()>() * V;
         const int extra = weight && few ? (cols + wide - 1) / wide : 0;
         auto kernel = few ? layer_norm_bwd_kernel<T, W, V, L, N, true> : layer_norm_bwd_kernel<T, W, V, L, N, false>;
