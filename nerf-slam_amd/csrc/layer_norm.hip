@@ -50,8 +50,8 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2]) {
 
 // columns [c, c + V) of a piece and how many of them the piece before it owns: the last piece of a row ends with the row and overlaps its
 // neighbour where D is no multiple of V.  Both lanes form and store the same bits there; a row's sums leave the first `skip` out.  skip >= V:
-// no piece (its lane reads the last one).  Pieces cut off element by element cost more (32768 x 1500 bf16: forward 53 instead of 38 us, backward 106 instead of 63).
-// whole: known not to be the last.
+// no piece (its lane reads the last one).  Pieces cut off element by element cost more (32768 x 1500 bf16: forward 53 instead of 38 us,
+// backward 106 instead of 63).  whole: known not to be the last.
 template <int V>
 __device__ __forceinline__ void ln_piece(int piece, int D, int& c, int& skip, bool whole = false) {
   c = whole ? piece * V : min(piece * V, D - V);
