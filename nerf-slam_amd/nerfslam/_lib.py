@@ -49,10 +49,17 @@ def _load(path):
     L.ns_ngp_encode_backward_fused_workspace_bytes.restype = C.c_size_t
     L.ns_ba_solve_large_workspace_bytes.restype = C.c_size_t
     L.ns_ngp_mlp_fragment_table_bytes.restype = C.c_size_t
-    L.ns_embedding_backward_workspace_bytes.restype = C.c_size_t
-    L.ns_embedding_backward_workspace_bytes.argtypes = [C.c_long, C.c_long, C.c_int, C.c_int]
-    L.ns_layer_norm_backward_workspace_bytes.restype = C.c_size_t
-    L.ns_layer_norm_backward_workspace_bytes.argtypes = [C.c_long, C.c_int, C.c_int]
+    # (the row operators' calls take a few microseconds: with their types declared ctypes converts plain numbers and addresses itself)
+    vp, lg, it, fl, sz = C.c_void_p, C.c_long, C.c_int, C.c_float, C.c_size_t
+    for name, res, args in (
+            ("ns_embedding_forward", it, [vp, lg, vp, it, vp, it, lg, lg, it, fl, vp]),
+            ("ns_embedding_backward_workspace_bytes", sz, [lg, lg, it, it]),
+            ("ns_embedding_backward", it, [vp, lg, it, vp, it, vp, it, lg, lg, it, fl, vp, sz, vp]),
+            ("ns_layer_norm_forward", it, [vp, lg, vp, vp, it, vp, vp, vp, it, lg, it, fl, vp]),
+            ("ns_layer_norm_backward_workspace_bytes", sz, [lg, it, it]),
+            ("ns_layer_norm_backward", it, [vp, lg, vp, lg, vp, vp, vp, it, vp, vp, vp, it, lg, it, vp, sz, vp])):
+        f = getattr(L, name)
+        f.restype, f.argtypes = res, args
     return L
 
 

@@ -7,12 +7,11 @@ collapse to one stride; outputs are fresh dense tensors.  Sums are f32, every ou
 explicit, as the trainer's are: nothing here records on torch's autograd tape.  Launches go to torch's current stream of the tensors'
 device, nothing synchronises, and every call has its own workspace, so calls may be captured into HIP graphs and run on several streams.
 """
-import ctypes as C
 import functools
 
 import torch
 
-from ._lib import NerfSlamHipError, check, lib, ptr, require_cuda
+from ._lib import NerfSlamHipError, check, lib, require_cuda
 
 _DT = {torch.float16: 1, torch.float32: 2, torch.bfloat16: 3}
 
@@ -31,13 +30,17 @@ def _same_device(op, first, *others):
     return device
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _call(name, what, device, *args):
     """the entry point `name` on the current stream of `device`"""
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
             return _call(name, what, device, *args)
     # (the stream's handle without building torch's Stream object: 0.1 us instead of 3.4, of calls that take 3 us on the device)
-    check(getattr(lib(), name)(*args, C.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))), what)
+    check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(device.index)), what)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -53,6 +56,8 @@ def _rows_of(op, name, t):
     if t.dim() < 1:
         _fail(op, f"{name} needs at least one axis")
     cols = t.shape[-1]
+    if cols > 65536:
+        _fail(op, f"{name} has rows of {cols} elements: at most 65536 are supported")
     if cols and t.is_contiguous():
         return t.numel() // cols, cols
     n = 1
@@ -93,8 +98,8 @@ def embedding(table, ids, scale=1.0):
     cols = table.shape[1]
     out = table.new_empty((*ids.shape, cols))
     if out.numel():
-        _call("ns_embedding_forward", "embedding_forward", device, ptr(table), C.c_long(stride), ptr(ids), is64, ptr(out),
-              _DT[table.dtype], C.c_long(ids.numel()), C.c_long(rows), cols, C.c_float(scale))
+        _call("ns_embedding_forward", "embedding_forward", device, _ptr(table), stride, _ptr(ids), is64, _ptr(out),
+              _DT[table.dtype], ids.numel(), rows, cols, float(scale))
     return out
 
 
@@ -118,8 +123,8 @@ def embedding_backward(dout, ids, rows, scale=1.0, dtype=None):
     if grad.numel():
         nbytes = _workspace_bytes("ns_embedding_backward_workspace_bytes", n, rows, cols, _DT[dout.dtype])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        _call("ns_embedding_backward", op, device, ptr(dout), C.c_long(stride), _DT[dout.dtype], ptr(ids), is64, ptr(grad), _DT[dtype],
-              C.c_long(n), C.c_long(rows), cols, C.c_float(scale), ptr(ws), C.c_size_t(nbytes))
+        _call("ns_embedding_backward", op, device, _ptr(dout), stride, _DT[dout.dtype], _ptr(ids), is64, _ptr(grad), _DT[dtype],
+              n, rows, cols, float(scale), _ptr(ws), nbytes)
     return grad
 
 
@@ -151,8 +156,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=False):
     if stats:
         mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
         rstd = torch.empty_like(mean)
-    _call("ns_layer_norm_forward", "layer_norm_forward", device, ptr(x), C.c_long(stride), ptr(weight), ptr(bias), _DT[wdtype], ptr(y),
-          ptr(mean), ptr(rstd), _DT[x.dtype], C.c_long(n), x.shape[-1], C.c_float(eps))
+    _call("ns_layer_norm_forward", "layer_norm_forward", device, _ptr(x), stride, _ptr(weight), _ptr(bias), _DT[wdtype], _ptr(y),
+          _ptr(mean), _ptr(rstd), _DT[x.dtype], n, x.shape[-1], float(eps))
     return (y, mean, rstd) if stats else y
 
 
@@ -177,6 +182,6 @@ def layer_norm_backward(dout, x, mean, rstd, weight=None):
         dw, db = torch.empty_like(weight), torch.empty_like(weight)
         nbytes = _workspace_bytes("ns_layer_norm_backward_workspace_bytes", n, cols, _DT[x.dtype])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _call("ns_layer_norm_backward", op, device, ptr(dout), C.c_long(dstride), ptr(x), C.c_long(stride), ptr(mean), ptr(rstd), ptr(weight),
-          _DT[wdtype], ptr(dx), ptr(dw), ptr(db), _DT[x.dtype], C.c_long(n), cols, ptr(ws), C.c_size_t(nbytes))
+    _call("ns_layer_norm_backward", op, device, _ptr(dout), dstride, _ptr(x), stride, _ptr(mean), _ptr(rstd), _ptr(weight),
+          _DT[wdtype], _ptr(dx), _ptr(dw), _ptr(db), _DT[x.dtype], n, cols, _ptr(ws), nbytes)
     return dx, dw, db

@@ -42,6 +42,8 @@ def test_cpu_tensors_are_refused():
     (lambda x, i: rows.layer_norm(x, torch.ones(8)[::2]), "contiguous"),
     (lambda x, i: rows.layer_norm(torch.zeros(4, 6, 8)[:, :3].transpose(0, 1)), "constant stride"),
     (lambda x, i: rows.layer_norm(torch.tensor(1.0)), "axis"),
+    (lambda x, i: rows.layer_norm(torch.empty((1, 2 ** 32 + 4), device="meta")), "65536"),       # (not cut to 4 columns)
+    (lambda x, i: rows.embedding(torch.empty((3, 65537), device="meta"), i), "65536"),
     (lambda x, i: rows.layer_norm_backward(x.half(), x, torch.zeros(3), torch.zeros(3)), "does not match"),
     (lambda x, i: rows.layer_norm_backward(x[:2], x, torch.zeros(3), torch.zeros(3)), "does not match"),
     (lambda x, i: rows.layer_norm_backward(x, x, torch.zeros(4), torch.zeros(3)), "mean"),
