@@ -1,0 +1,122 @@
+"""Row operators (nerfslam/rows.py) where a bound that grows with the number of terms would let a lost term pass: sums of small whole
+numbers, which f32 holds exactly in any order, so that the answer is EQUAL to the 64-bit one or wrong.  No term is
+zero: leaving out any one of them changes every column it is in."""
+import pytest
+import torch
+
+from nerfslam import rows
+from test_rows_gpu import F16, F32, U, gen, half, make_ids, randn, tiny, within
+
+pytestmark = pytest.mark.gpu
+
+
+def whole(g, shape, most, dtype):
+    """whole numbers of either sign, 1 .. most in size"""
+    f = torch.randint(1, most + 1, shape, generator=g, device=g.device).float()
+    return (f * (torch.randint(0, 2, shape, generator=g, device=g.device) * 2 - 1)).to(dtype)
+
+
+def grad64(dout, ids, v):
+    """the gradient in 64 bits, and the sum of its terms' sizes.  Rows with many tokens are summed slice by slice of the sorted list: scattered
+    additions onto one row take the device minutes."""
+    s, a = (torch.zeros((v, dout.shape[-1]), dtype=torch.float64, device=ids.device) for _ in range(2))
+    key, order = torch.sort(torch.where((ids >= 0) & (ids < v), ids, torch.full_like(ids, v)).long())
+    count = torch.bincount(key, minlength=v + 1)[:v]
+    first = torch.cumsum(count, 0) - count
+    hot = torch.nonzero(count > 256)[:, 0]
+    for r, at, m in zip(hot.tolist(), first[hot].tolist(), count[hot].tolist()):
+        d = dout[order[at:at + m]].double()
+        s[r], a[r] = d.sum(0), d.abs().sum(0)
+    rest = key < v
+    rest[rest.clone()] = count[key[rest]] <= 256
+    key, d = key[rest], dout[order[rest]].double()
+    return s.index_add_(0, key, d), a.index_add_(0, key, d.abs())
+
+
+def check_whole(dout, ids, v):
+    want, size = grad64(dout, ids, v)
+    assert float(size.max() if size.numel() else 0.0) < 2.0 ** 24           # every partial sum is exact, whatever the order
+    for dtype in {F32, dout.dtype}:
+        got = rows.embedding_backward(dout, ids, v, scale=0.5, dtype=dtype)
+        assert torch.equal(got, (want * 0.5).float().to(dtype)), (tuple(dout.shape), v, dtype)
+
+
+def place(dev, counts, n, seed):
+    """n ids: counts[r] of row r, the rest padded places, in random order"""
+    ids = torch.full((n,), -1, dtype=torch.int64, device=dev)
+    at = 0
+    for r, m in counts:
+        ids[at:at + m] = r
+        at += m
+    assert at <= n
+    return ids[torch.randperm(n, generator=gen(dev, seed), device=dev)]
+
+
+# one row takes everything, or all but a few tokens: up to 4096 tokens in one launch; up to 1023 narrow rows as tiles' sums added per row;
+# else sorted, where the row's run crosses shares of the list: 4 .. 512 of them in these cases, beyond 64 found by search
+ONE = [(4096, 50, 771), (4096, 300000, 9), (8192, 10, 130), (8192, 1, 1000), (8192, 5000, 8), (12000, 2000, 1000), (16384, 1, 264), (33000, 1, 1000),
+       (70000, 9, 40), (100000, 300, 60), (300000, 1, 8), (1 << 20, 512, 16), (300000, 1024, 8), (100000, 1030, 60), (70000, 1024, 1), (140000, 3, 512)]
+
+
+@pytest.mark.parametrize("n,v,d", ONE)
+def test_one_row_takes_everything(dev, n, v, d):
+    g = gen(dev, n + v + d)
+    for dtype in (F16, F32):
+        dout = whole(g, (n, d), 8, dtype)
+        check_whole(dout, torch.full((n,), v // 2, dtype=torch.int32, device=dev), v)
+        ids = make_ids(g, n, v, "pad")                                       # a tenth padded or named by chance, the row the others
+        check_whole(dout, torch.where(torch.rand(n, generator=g, device=dev) < 0.9, torch.full_like(ids, v - 1), ids), v)
+
+
+@pytest.mark.parametrize("n,v,d", [(5000, 20, 12), (9000, 40, 300), (12000, 2000, 40), (33000, 1100, 1000), (100000, 1500, 60), (262144, 512, 32), (262144, 1500, 32)])
+def test_a_few_rows_take_most(dev, n, v, d):
+    """frequency ~ 1 / rank: runs of every length at once, next to each other in the sorted list"""
+    g = gen(dev, n + d)
+    dout = whole(g, (n, d), 4, F16)
+    for kind in ("skew", "sorted", "pad"):
+        check_whole(dout, make_ids(g, n, v, kind), v)
+    ids = make_ids(g, n, v, "skew")
+    check_whole(dout, torch.where(ids < 3, ids, torch.full_like(ids, -1)), v)
+
+
+@pytest.mark.parametrize("behind", ["row", "padding", "nothing"])
+@pytest.mark.parametrize("before", [0, 1, 100, 255, 256])
+def test_runs_that_end_at_the_borders_of_shares(dev, before, behind):
+    """1000 f16 columns, 33000 tokens: shares of 256 places.  A run that crosses 1, 2, 63 .. 67 shares' ends, ending just before, at and
+    behind such an end; the search for the end of a run begins where 64 shares' beginnings have been looked at"""
+    n, v, d = 33000, 1, 1000
+    dout = whole(gen(dev, before), (n, d), 8, F16)
+    lengths = [m * 256 + k for m in (1, 2, 63, 64, 65, 66, 67) for k in (-1, 0, 1)]
+    for i, m in enumerate(lengths if behind != "nothing" else [n - before]):
+        counts = [(0, before), (1, m)] + ([(2, n - before - m)] if behind == "row" else [])
+        check_whole(dout, place(dev, counts, n, i), 3)
+
+
+@pytest.mark.parametrize("n", [530001, 1100000])
+def test_more_than_1024_shares(dev, n):
+    """264 and 257 f16 columns: shares of 512 places, 1036 and 2149 of them, so that a workgroup of the join looks at two and at three"""
+    d = 264 if n == 530001 else 257
+    g = gen(dev, n)
+    dout = whole(g, (n, d), 4, F16)
+    ids = make_ids(g, n, 3000, "skew", torch.int32)
+    check_whole(dout, ids, 3000)
+    check_whole(dout, torch.where(torch.rand(n, generator=g, device=dev) < 0.6, torch.full_like(ids, 1), ids), 3000)      # (600 shares of one row)
+    check_whole(dout, torch.randint(0, 5, (n,), generator=g, device=dev), 5)
+
+
+@pytest.mark.parametrize("n,v,d,kind", [
+    (300000, 1, 8, "one"), (70000, 9, 40, "one"), (100000, 300, 60, "one"), ((1 << 20) + 5, 512, 8, "skew"), (1 << 20, 512, 16, "even"), (33000, 1, 1000, "one"),
+    (300000, 1030, 8, "one"), (140000, 2, 512, "one"), (4096, 3, 771, "one"), (8192, 3, 130, "one")])
+def test_embedding_backward_by_the_length_of_its_chains(dev, n, v, d, kind):
+    """The longest chain of additions, whatever the number of tokens of a row: at most 128 places in a lane, then 6 steps across a wave and
+    16 waves, then the partial rows: 256 sub-groups that each add every 256th (1 lane per row), or 4 that each add every 4th of
+    n / 512 (64 lanes) -- below 128 + 6 + 16 + 256 + n / 2048 + 4 links.  A row of 300000 tokens of size 0.8 may then be off by 8; its sums
+    are 550 in size, a lost group of 64 tokens 8."""
+    g = gen(dev, v + d)
+    ids, dout = make_ids(g, n, v, kind), randn(g, n, d)
+    want, size = grad64(dout, ids, v)
+    links = 410 + n / 2048
+    tol = links * U * size * 0.5 + (half(F32) + U) * want.abs() + tiny(F32)
+    within(rows.embedding_backward(dout, ids, v, scale=0.5), want * 0.5, tol, (n, v, d, kind))
+    if kind == "one":
+        assert bool((want.abs()[v // 2] * 0.5 > tol[v // 2]).float().mean() > 0.8)           # (zeros would not pass)
