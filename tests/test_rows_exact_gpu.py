@@ -1,11 +1,11 @@
 """Row operators (nerfslam/rows.py) where a bound that grows with the number of terms would let a lost term pass: sums of small whole
-numbers, which f32 holds exactly in any order, so that the answer is EQUAL to the 64-bit one or wrong.  No term is
-zero: leaving out any one of them changes every column it is in."""
+numbers, which f32 holds exactly in any order, so that the answer is EQUAL to the 64-bit one or wrong; and random rows by the thousand
+against 64 bits for every shape of the norm's row loop.  No term is zero: leaving out any one of them changes every column it is in."""
 import pytest
 import torch
 
 from nerfslam import rows
-from test_rows_gpu import F16, F32, U, gen, half, make_ids, randn, tiny, within
+from test_rows_gpu import BF16, F16, F32, U, check_norm, check_norm_backward, gen, half, make_ids, norm64, randn, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,34 @@ def test_embedding_backward_by_the_length_of_its_chains(dev, n, v, d, kind):
     within(rows.embedding_backward(dout, ids, v, scale=0.5), want * 0.5, tol, (n, v, d, kind))
     if kind == "one":
         assert bool((want.abs()[v // 2] * 0.5 > tol[v // 2]).float().mean() > 0.8)           # (zeros would not pass)
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+# every shape of the row loop, with more rows than its workgroups take in one turn
+@pytest.mark.parametrize("n,d,dtype", [
+    (300000, 3, F32), (270000, 32, F32), (140000, 60, F32), (70001, 128, F32), (40000, 250, F32), (40000, 500, F32), (20000, 771, F32), (10000, 1000, F32),
+    (6000, 2000, F32), (3000, 4096, F32), (700, 8192, F32), (700, 16384, F32), (600, 9001, F32),
+    (270000, 64, BF16), (9000, 2048, BF16), (5000, 4000, F16), (1300, 8192, BF16), (1300, 16384, F16), (1300, 16384, BF16)])
+def test_norm_of_many_rows_both_ways(dev, n, d, dtype):
+    g = gen(dev, n + d)
+    x = (1.5 * randn(g, n, d) + 0.5 * randn(g, 1, d) + 0.3).to(dtype)
+    w, b = 1.0 + 0.1 * randn(g, d), 0.1 * randn(g, d)
+    check_norm(rows.layer_norm(x, w, b, stats=True), x, w, b, 1e-5, (n, d, dtype))
+    _, mean, rstd = norm64(x, None, None, 1e-5)                              # (not the kernel's own)
+    mean, rstd, dout = mean.float(), rstd.float(), randn(g, n, d, dtype=dtype)
+    check_norm_backward(rows.layer_norm_backward(dout, x, mean, rstd, w), dout, x, mean, rstd, w, (n, d, dtype))
+
+
+@pytest.mark.parametrize("n,d,dtype,wdtype", [
+    (1, 5, F32, F32), (33, 1024, BF16, F32), (512, 771, F32, F32), (511, 16384, F16, F32), (513, 3, F16, F16), (513, 771, F32, F32), (2500, 771, F32, F32),
+    (100000, 16, F16, F32), (70001, 128, F16, F32), (230400, 128, F16, F32), (40000, 500, F32, F32), (9000, 1024, BF16, BF16), (3001, 4096, BF16, F32),
+    (3000, 4096, F32, F32), (1300, 16384, F16, F16), (700, 16384, F32, F32)])
+def test_weight_gradients_lose_no_row(dev, n, d, dtype, wdtype):
+    """mean 0 and rstd 1 as given statistics: dweight = sum dout x, dbias = sum dout, of whole numbers"""
+    g = gen(dev, n * 3 + d)
+    x, dout = whole(g, (n, d), 3, dtype), whole(g, (n, d), 3, dtype)
+    mean, rstd = torch.zeros(n, device=dev), torch.ones(n, device=dev)
+    assert 9 * n < 2 ** 24
+    _, dw, db = rows.layer_norm_backward(dout, x, mean, rstd, whole(g, (d,), 2, wdtype))
+    assert torch.equal(dw, (dout.double() * x.double()).sum(0).float().to(wdtype))
+    assert torch.equal(db, dout.double().sum(0).float().to(wdtype))
