@@ -764,8 +764,8 @@ int ns_embedding_backward(const void* dout, long dout_stride, int dtype, const v
 int ns_layer_norm_forward(const void* x, long x_stride, const void* weight, const void* bias, int wdtype, void* y, float* mean,
                           float* rstd, int dtype, long n, int cols, float eps, void* stream);
 /* With g = dy * weight and xh = (x - mean) * rstd:  dx = rstd * (g - mean(g) - xh * mean(g xh)), dweight = sum over rows of dy xh,
- * dbias = sum over rows of dy (both of wdtype, in a fixed order).  weight, dweight and dbias: all or none (none: dx alone).
- *   ws: ns_layer_norm_backward_workspace_bytes(n, cols, dtype) bytes (none without a weight; 0 for few rows), as above.        */
+ * dbias = sum over rows of dy (both of wdtype, in a fixed order).  weight and dweight: both or neither; dbias with or without them.
+ *   ws: ns_layer_norm_backward_workspace_bytes(n, cols, dtype) bytes (none for dx alone; 0 for few rows), as above.            */
 size_t ns_layer_norm_backward_workspace_bytes(long n, int cols, int dtype);
 int ns_layer_norm_backward(const void* dy, long dy_stride, const void* x, long x_stride, const float* mean, const float* rstd,
                            const void* weight, int wdtype, void* dx, void* dweight, void* dbias, int dtype, long n, int cols, void* ws,

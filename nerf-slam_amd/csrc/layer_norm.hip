@@ -127,7 +127,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T
 }
 
 // ---------------------------------------------------------------------------------------------
-// backward.  part: [workgroups][2][D] f32 (dw | db), or nullptr: no weight.
+// backward.  part: [workgroups][2][D] f32 (dw | db), or nullptr: neither is asked for.  dweight / dbias: nullptr where that one is not.
 //
 // FEW: few rows, one launch, no part.  The weight gradients are formed by further workgroups (from row_blocks on), ln_columns pieces of the
 // columns each over all rows, which are read a second time (they lie in the caches): dw and db need no sum over a row, mean and rstd are given.
@@ -177,7 +177,8 @@ __device__ __forceinline__ void layer_norm_columns(const T* __restrict__ dy, lon
 #pragma unroll
       for (int q = 0; q < WAVES; q++) acc[i] += red[((q * 2 + k) * COLUMNS + piece) * V + i];
     }
-    if (skip < V) row_put<W, V, false>((k ? dbias : dweight) + c, acc);
+    W* out = k ? dbias : dweight;
+    if (skip < V && out) row_put<W, V, false>(out + c, acc);
   }
 }
 
@@ -270,7 +271,8 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
   }
   if (FEW || !part) return;
 #pragma unroll
-  for (int k = 0; k < 2; k++)
+  for (int k = 0; k < 2; k++) {
+    if (!(k ? dbias : dweight)) continue;                        // (that half is not read)
 #pragma unroll
     for (int j = 0; j < NV; j++) {
       float(&acc)[V] = k ? db[j] : dw[j];
@@ -288,6 +290,7 @@ __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_bwd_kernel(const T
       }
       if (threadIdx.x < LPR && skip[j] < V) row_put<float, V, false>(part + ((long)blockIdx.x * 2 + k) * D + c[j], acc);
     }
+  }
 }
 
 // dw | db [2 D] from the workgroups' partial rows: COLS columns per workgroup, 1024 / COLS groups of lanes share the rows and meet through
@@ -299,8 +302,9 @@ __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __r
   __shared__ float red[16][COLS];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int c = blockIdx.x * COLS + lane % COLS;
+  const bool asked = c < 2 * D && (c < D ? dw : db);
   float s = 0.0f;
-  if (c < 2 * D) {
+  if (asked) {
 #pragma unroll 8
     for (int i = threadIdx.x / COLS; i < parts; i += 1024 / COLS) s += part[(long)i * 2 * D + c];
   }
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __r
   for (int o = COLS; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
   if (lane < COLS) red[wv][lane] = s;
   __syncthreads();
-  if (threadIdx.x < COLS && c < 2 * D) {
+  if (threadIdx.x < COLS && asked) {
     s = red[0][lane];
 #pragma unroll
     for (int i = 1; i < 16; i++) s += red[i][lane];
@@ -420,9 +424,9 @@ extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void
   NS_REQUIRE(n >= 0 && n <= (1L << 40) && cols >= 1 && cols <= LN_MAX_COLS && x_stride >= 0 && dy_stride >= 0,
              "ns_layer_norm_backward: bad shape (n %ld, cols %d in 1 .. %d)", n, cols, LN_MAX_COLS);
   NS_REQUIRE(n == 0 || (dy && x && mean && rstd && dx), "ns_layer_norm_backward: null pointer");
-  NS_REQUIRE((weight != nullptr) == (dweight != nullptr) && (weight != nullptr) == (dbias != nullptr),
-             "ns_layer_norm_backward: weight, dweight and dbias come together");
-  const size_t need = weight ? ns_layer_norm_backward_workspace_bytes(n, cols, dtype) : 0;
+  NS_REQUIRE((weight != nullptr) == (dweight != nullptr), "ns_layer_norm_backward: weight and dweight come together");
+  const bool sums = dweight || dbias;
+  const size_t need = sums ? ns_layer_norm_backward_workspace_bytes(n, cols, dtype) : 0;
   NS_REQUIRE(ws_bytes >= need && (ws || need == 0), "ns_layer_norm_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
   NS_REQUIRE(row_aligned(dy, dtype) && row_aligned(x, dtype) && row_aligned(dx, dtype) && row_aligned(weight, wdtype) &&
                  row_aligned(dweight, wdtype) && row_aligned(dbias, wdtype) && row_aligned(mean, NS_F32) && row_aligned(rstd, NS_F32) &&
@@ -433,19 +437,19 @@ extern "C" int ns_layer_norm_backward(const void* dy, long dy_stride, const void
     using T = decltype(t);
     using W = decltype(u);
     const bool few = n <= LN_FEW_ROWS;
-    if (n > 0 || (weight && few))
+    if (n > 0 || (sums && few))
       ln_shape<row_vec<T>()>(cols, [&](auto vec, auto lpr, auto nv) {
         constexpr int V = decltype(vec)::v, L = decltype(lpr)::v, N = decltype(nv)::v, wide = ln_columns<ln_block<L>()>() * V;
-        const int extra = weight && few ? (cols + wide - 1) / wide : 0;
+        const int extra = sums && few ? (cols + wide - 1) / wide : 0;
         auto kernel = few ? layer_norm_bwd_kernel<T, W, V, L, N, true> : layer_norm_bwd_kernel<T, W, V, L, N, false>;
         hipLaunchKernelGGL(kernel, dim3(blocks + extra), dim3(ln_block<L>()), 0, (hipStream_t)stream, (const T*)dy, dy_stride, (const T*)x,
-                           x_stride, mean, rstd, (const W*)weight, (T*)dx, weight ? (float*)ws : nullptr, (W*)dweight, (W*)dbias, n, cols,
+                           x_stride, mean, rstd, (const W*)weight, (T*)dx, sums ? (float*)ws : nullptr, (W*)dweight, (W*)dbias, n, cols,
                            1.0f / (float)cols, blocks);
       });
-    if (weight && !few && cols <= 1024)
+    if (sums && !few && cols <= 1024)
       hipLaunchKernelGGL((layer_norm_wgrad_kernel<W, 16>), dim3((2 * cols + 15) / 16), dim3(1024), 0, (hipStream_t)stream, (const float*)ws,
                          blocks, cols, (W*)dweight, (W*)dbias);
-    else if (weight && !few)
+    else if (sums && !few)
       hipLaunchKernelGGL((layer_norm_wgrad_kernel<W, 64>), dim3((2 * cols + 63) / 64), dim3(1024), 0, (hipStream_t)stream, (const float*)ws,
                          blocks, cols, (W*)dweight, (W*)dbias);
   });

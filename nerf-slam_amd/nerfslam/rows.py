@@ -136,12 +136,8 @@ def _weight(op, x, name, t):
     return t.dtype
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=False):
-    """(x - mean) * rstd * weight + bias over the last axis (at most 16384 wide), rstd = 1 / sqrt(var + eps) with the biased variance;
-    weight / bias [D] in x's dtype or float32, each may be None.  stats=True: (y, mean, rstd), the latter two float32 of x.shape[:-1] --
-    what `layer_norm_backward` takes."""
-    op = "layer_norm"
-    n, stride = _rows_of(op, "x", x)
+def _weights(op, x, weight, bias):
+    """the dtype of weight and bias, each may be None"""
     wdtype = torch.float32
     if weight is not None:
         wdtype = _weight(op, x, "weight", weight)
@@ -150,6 +146,16 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=False):
         if weight is not None and bdtype != wdtype:
             _fail(op, "weight and bias have to be of one dtype")
         wdtype = bdtype
+    return wdtype
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=False):
+    """(x - mean) * rstd * weight + bias over the last axis (at most 16384 wide), rstd = 1 / sqrt(var + eps) with the biased variance;
+    weight / bias [D] in x's dtype or float32, each may be None.  stats=True: (y, mean, rstd), the latter two float32 of x.shape[:-1] --
+    what `layer_norm_backward` takes."""
+    op = "layer_norm"
+    n, stride = _rows_of(op, "x", x)
+    wdtype = _weights(op, x, weight, bias)
     device = _same_device(op, x, weight, bias)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = None
@@ -161,9 +167,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=False):
     return (y, mean, rstd) if stats else y
 
 
-def layer_norm_backward(dout, x, mean, rstd, weight=None):
+def layer_norm_backward(dout, x, mean, rstd, weight=None, bias=None):
     """gradients of `layer_norm` from the upstream gradient dout (x's shape and dtype) and what the forward pass saved:
-    (dx, dweight, dbias) -- dx in x's dtype, the other two in the weight's; (dx, None, None) without a weight."""
+    (dx, dweight, dbias) -- dx in x's dtype, the other two in the weight's or the bias'.  A weight alone gives both (dbias takes no further
+    pass); a bias alone, of which only dtype and shape count, (dx, None, dbias); neither (dx, None, None)."""
     op = "layer_norm_backward"
     n, stride = _rows_of(op, "x", x)
     if dout.dtype != x.dtype or dout.shape != x.shape:
@@ -172,14 +179,15 @@ def layer_norm_backward(dout, x, mean, rstd, weight=None):
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous():
             _fail(op, f"{name} must be a contiguous float32 {tuple(x.shape[:-1])} tensor")
-    wdtype = torch.float32 if weight is None else _weight(op, x, "weight", weight)
-    device = _same_device(op, x, dout, mean, rstd, weight)
+    wdtype = _weights(op, x, weight, bias)
+    device = _same_device(op, x, dout, mean, rstd, weight, bias)
     cols = x.shape[-1]
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = db = ws = None
     nbytes = 0
-    if weight is not None:
-        dw, db = torch.empty_like(weight), torch.empty_like(weight)
+    if weight is not None or bias is not None:
+        db = torch.empty_like(bias if weight is None else weight)
+        dw = None if weight is None else torch.empty_like(weight)
         nbytes = _workspace_bytes("ns_layer_norm_backward_workspace_bytes", n, cols, _DT[x.dtype])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _call("ns_layer_norm_backward", op, device, _ptr(dout), dstride, _ptr(x), stride, _ptr(mean), _ptr(rstd), _ptr(weight),

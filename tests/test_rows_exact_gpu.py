@@ -1,10 +1,13 @@
 """Row operators (nerfslam/rows.py) where a bound that grows with the number of terms would let a lost term pass: sums of small whole
 numbers, which f32 holds exactly in any order, so that the answer is EQUAL to the 64-bit one or wrong; and random rows by the thousand
 against 64 bits for every shape of the norm's row loop.  No term is zero: leaving out any one of them changes every column it is in."""
+import ctypes as C
+
 import pytest
 import torch
 
 from nerfslam import rows
+from nerfslam._lib import check, lib, ptr, stream_ptr
 from test_rows_gpu import BF16, F16, F32, U, check_norm, check_norm_backward, gen, half, make_ids, norm64, randn, tiny, within
 
 pytestmark = pytest.mark.gpu
@@ -151,3 +154,59 @@ def test_weight_gradients_lose_no_row(dev, n, d, dtype, wdtype):
     _, dw, db = rows.layer_norm_backward(dout, x, mean, rstd, whole(g, (d,), 2, wdtype))
     assert torch.equal(dw, (dout.double() * x.double()).sum(0).float().to(wdtype))
     assert torch.equal(db, dout.double().sum(0).float().to(wdtype))
+
+
+@pytest.mark.parametrize("n,d,dtype,wdtype", [(7, 40, F32, F32), (300, 771, F16, F32), (512, 5000, BF16, BF16), (700, 33, F16, F16), (5000, 128, F32, F32), (600, 2050, BF16, F32), (0, 24, F32, F32)])
+def test_gradients_with_and_without_weight_and_bias(dev, n, d, dtype, wdtype):
+    """all four forms that the forward pass takes: dx against the formula, dweight and dbias each where it is asked for, and the same bits
+    with and without the other"""
+    g = gen(dev, n + d)
+    x, dout = (1.5 * randn(g, n, d) + 0.3).to(dtype), randn(g, n, d, dtype=dtype)
+    w, b = (1.0 + 0.1 * randn(g, d)).to(wdtype), (0.1 * randn(g, d)).to(wdtype)
+    _, mean, rstd = rows.layer_norm(x, w, b, stats=True)
+    both = rows.layer_norm_backward(dout, x, mean, rstd, w, b)
+    check_norm_backward(both, dout, x, mean, rstd, w, (n, d, "both"))
+    alone = rows.layer_norm_backward(dout, x, mean, rstd, w)
+    assert all(torch.equal(p, q) for p, q in zip(both, alone))
+    dx, dw, db = rows.layer_norm_backward(dout, x, mean, rstd, None, b)
+    check_norm_backward((dx, None, None), dout, x, mean, rstd, None, (n, d, "bias"))
+    assert dw is None and db.dtype == wdtype and torch.equal(db, both[2])
+    plain = rows.layer_norm_backward(dout, x, mean, rstd)
+    assert torch.equal(plain[0], dx) and plain[1] is None and plain[2] is None
+
+
+@pytest.mark.parametrize("weight,bias", [(True, True), (True, False), (False, True), (False, False)])
+def test_gradients_of_each_form_against_autograd(dev, weight, bias):
+    """torch's own layer norm in 64 bits on the CPU.  f32 in and out: each output is within a few hundred u of the largest of its kind
+    (K links of a row sum, n / 128 + 305 of a column), 2^-13 leaves a factor of ten"""
+    g = gen(dev, 21)
+    x, dout = 1.5 * randn(g, 600, 100) + 0.3, randn(g, 600, 100)
+    w, b = (1.0 + 0.1 * randn(g, 100) if weight else None), (0.1 * randn(g, 100) if bias else None)
+    y, mean, rstd = rows.layer_norm(x, w, b, stats=True)
+    got = (y, *rows.layer_norm_backward(dout, x, mean, rstd, w, b))
+    x64, w64, b64 = (None if t is None else t.double().cpu().requires_grad_(True) for t in (x, w, b))
+    y64 = torch.nn.functional.layer_norm(x64, (100,), w64, b64, 1e-5)
+    (y64 * dout.double().cpu()).sum().backward()
+    for name, have, want in zip(("y", "dx", "dw", "db"), got, (y64.detach(), x64.grad, None if w64 is None else w64.grad, None if b64 is None else b64.grad)):
+        if want is not None:
+            within(have.cpu(), want, 2.0 ** -13 * float(want.abs().max()), name)
+
+
+def test_a_bias_alone_writes_nothing_else(dev):
+    """through the C ABI: dbias in the middle of a larger buffer, no dweight; and a weight without dbias"""
+    g, f, L = gen(dev, 22), lib(), C.c_long
+    for n, d in ((37, 33), (600, 40), (3000, 1500)):
+        x, dout = randn(g, n, d, dtype=F16), randn(g, n, d, dtype=F16)
+        w = randn(g, d)
+        _, mean, rstd = rows.layer_norm(x, w, stats=True)
+        need = f.ns_layer_norm_backward_workspace_bytes(L(n), d, 1)
+        for weight in (None, w):
+            ws = torch.full((need + 256,), 0x5a, dtype=torch.uint8, device=dev)
+            sums, dx = torch.full((d + 130,), 7.0, device=dev), torch.empty_like(x)
+            p = C.c_void_p(sums.data_ptr() + 65 * 4)
+            check(f.ns_layer_norm_backward(ptr(dout), L(d), ptr(x), L(d), ptr(mean), ptr(rstd), ptr(weight), 2, ptr(dx),
+                                           None if weight is None else p, p if weight is None else None, 1, L(n), d, ptr(ws), C.c_size_t(need),
+                                           stream_ptr()), "norm_bwd")
+            want = rows.layer_norm_backward(dout, x, mean, rstd, weight, w)
+            assert torch.equal(dx, want[0]) and torch.equal(sums[65:65 + d], want[2] if weight is None else want[1])
+            assert bool((sums[:65] == 7).all()) and bool((sums[65 + d:] == 7).all()) and bool((ws[need:] == 0x5a).all())
