@@ -752,7 +752,8 @@ int ns_embedding_forward(const void* table, long table_stride, const void* ids, 
                          int cols, float scale, void* stream);
 /* grad[r] = scale * sum of dout[t] over the tokens t with ids[t] == r; every row of grad [rows, cols] is written (0 without tokens),
  * rows of dout whose id lies outside [0, rows) are not used.  grad_dtype: dtype or NS_F32.  The tokens are sorted by id on the device
- * and the sums run over the sorted list in a fixed order: the same inputs give the same bits.  rows * ceil(cols / 256) <= 2^27.
+ * and the sums run over the sorted list in a fixed order: the same inputs give the same bits.  rows * ceil(cols / 256) <= 2^27; n <= 2^25,
+ * with more than 65280 f32 columns n <= 2^25 - 512.
  *   ws: ns_embedding_backward_workspace_bytes(n, rows, cols, dtype) bytes (0 for short lists, at most about 4 per element of dout + 16
  *   per token), 16-byte aligned, contents irrelevant; calls that may be in flight at the same time must not share it.          */
 size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols, int dtype);

@@ -881,25 +881,29 @@ __global__ __launch_bounds__(1024) void embed_small_kernel(const T* __restrict__
 // ---------------------------------------------------------------------------------------------
 // C ABI
 // ---------------------------------------------------------------------------------------------
-// limits that keep every grid below 2^32 threads (up to 64 lanes per token, 16 per table row and piece of its columns) and places in
-// 32 bits
+// limits that keep every grid below 2^32 threads (up to 64 lanes per token, 16 per table row and piece of its columns; the sums' grid by
+// EmbPlan::sums) and places in 32 bits
 #define EMB_MAX_COLS 65536
 #define EMB_MAX_TOKENS (1L << 25)
 #define EMB_MAX_ROW_PIECES (1L << 27)     // rows x ceil(columns / 256) of a gradient
+#define EMB_MAX_SUMS ((1L << 24) - 1)     // workgroups of 256 threads: only 2^25 tokens of more than 65280 f32 columns pass it
 
 // small: group = rows per workgroup, shares = pieces of the columns
 struct EmbPlan {
   bool small, ranked, few;
   int passes, bits, tiles, ls, group, shares;
+  long sums;       // workgroups of embed_sum_kernel (general form)
   size_t keys[2], order[2], hist, total, part, touched, bytes;
 };
+
+static inline int emb_col_blocks(int cols, int vec, int ls) { return (cols + (vec << ls) - 1) / (vec << ls); }
 
 static EmbPlan emb_plan(long n, long rows, int cols, int vec) {
   EmbPlan p = {};
   p.ls = row_lanes_log2(cols, vec);
   if (n <= SMALL_MAX) {
     // narrow pieces of the columns: a row that takes most of the tokens is still the work of several workgroups
-    const int ls = p.ls < SMALL_LANES ? p.ls : SMALL_LANES, pieces = (cols + (vec << ls) - 1) / (vec << ls);
+    const int ls = p.ls < SMALL_LANES ? p.ls : SMALL_LANES, pieces = emb_col_blocks(cols, vec, ls);
     int own = 1;                                             // rows per workgroup
     while (own < SMALL_ROWS && (rows + own - 1) / own * pieces > SMALL_BLOCKS) own *= 2;
     if (n == 0 || (rows + own - 1) / own * pieces <= 4 * SMALL_BLOCKS) {
@@ -938,6 +942,7 @@ static EmbPlan emb_plan(long n, long rows, int cols, int vec) {
     p.keys[i] = take(i == 0 || p.passes > 1 ? 4 * (size_t)n : 0);
     p.order[i] = take(i == 0 || p.passes > 1 ? 4 * (size_t)n : 0);
   }
+  p.sums = (long)p.shares * emb_col_blocks(cols, vec, p.ls);
   p.hist = take(n <= ONE_MAX ? 0 : (size_t)p.tiles * (4u << p.bits));
   p.total = take(n <= ONE_MAX ? 0 : 4u << p.bits);
   p.part = take(p.shares > 1 ? (size_t)p.shares * 2 * cols * 4 : 0);
@@ -1004,7 +1009,8 @@ extern "C" int ns_embedding_forward(const void* table, long table_stride, const 
 
 extern "C" size_t ns_embedding_backward_workspace_bytes(long n, long rows, int cols, int dtype) {
   if (n <= 0 || rows <= 0 || !emb_fits(n, rows, cols)) return 0;
-  return emb_plan(n, rows, cols, emb_vec(dtype, cols)).bytes;
+  const EmbPlan p = emb_plan(n, rows, cols, emb_vec(dtype, cols));
+  return p.sums <= EMB_MAX_SUMS ? p.bytes : 0;
 }
 
 template <typename I>
@@ -1079,7 +1085,7 @@ static void emb_few(const EmbPlan& p, const T* dout, long dstride, const I* ids,
 template <typename T, int V, typename G>
 static void emb_sums(const EmbPlan& p, const T* dout, long dstride, const unsigned* keys, const int* order, int n, unsigned rows,
                      int cols, float scale, G* grad, float* part, hipStream_t s) {
-  const int col_blocks = (cols + (V << p.ls) - 1) / (V << p.ls), share = p.group * (256 >> p.ls);
+  const int col_blocks = emb_col_blocks(cols, V, p.ls), share = p.group * (256 >> p.ls);
   hipLaunchKernelGGL((embed_sum_kernel<T, V, G>), dim3((unsigned)p.shares * col_blocks), dim3(256), 0, s, dout, dstride, keys, order, n, rows,
                      cols, p.ls, p.group, col_blocks, scale, grad, part);
   if (p.shares > 1) {
@@ -1102,6 +1108,7 @@ extern "C" int ns_embedding_backward(const void* dout, long dout_stride, int dty
              "ns_embedding_backward: bad shape (n %ld <= 2^25, cols %d in 1 .. %d, rows %ld x ceil(cols / 256) <= 2^27)", n, cols, EMB_MAX_COLS,
              rows);
   const EmbPlan p = emb_plan(n, rows, cols, emb_vec(dtype, cols));
+  NS_REQUIRE(p.sums <= EMB_MAX_SUMS, "ns_embedding_backward: bad shape (n %ld of %d f32 columns: n <= 2^25 - 512 beyond 65280 columns)", n, cols);
   NS_REQUIRE(grad && (n == 0 || (dout && ids)) && (ws || p.bytes == 0), "ns_embedding_backward: null pointer");
   NS_REQUIRE(ws_bytes >= p.bytes, "ns_embedding_backward: workspace of %zu bytes, %zu needed", ws_bytes, p.bytes);
   NS_REQUIRE(((uintptr_t)ws % 16) == 0, "ns_embedding_backward: the workspace needs 16-byte alignment");

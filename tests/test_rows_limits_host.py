@@ -33,3 +33,16 @@ def test_a_bias_alone_is_checked_as_a_weight_is():
     _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, P, P, 2, P, None, None, 2, L(3), 4, P, C.c_size_t(0), None), "together")
     _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, P, None, 2, P, P, None, 2, L(3), 4, P, C.c_size_t(0), None), "together")
     _refused(f.ns_layer_norm_backward(P, L(4), P, L(4), P, P, None, 2, P, None, C.c_void_p(4097), 2, L(3), 4, P, C.c_size_t(0), None), "aligned")
+
+
+def test_the_largest_gradients_grids():
+    """f32 rows of 65536 columns, 2^25 of them (one row expanded along the leading axis): the sums' grid would have 65536 shares x 256 pieces of the
+    columns x 256 threads = 2^32 threads, one more than a launch takes.  Refused by its shape; the neighbours are sized as before."""
+    f, big, z = lib(), C.c_size_t(1 << 60), C.c_size_t(0)
+    size = f.ns_embedding_backward_workspace_bytes
+    for n, cols in ((1 << 25, 65536), (1 << 25, 65281), ((1 << 25) - 511, 65536)):
+        _refused(f.ns_embedding_backward(P, L(0), 2, P, 0, P, 2, L(n), L(1), cols, C.c_float(1), P, big, None), "2^25 - 512")
+        assert size(L(n), L(1), cols, 2) == 0
+    for n, cols, dtype in (((1 << 25) - 512, 65536, 2), (1 << 25, 65280, 2), (1 << 25, 65536, 1), (1 << 25, 65536, 3)):
+        assert size(L(n), L(1), cols, dtype) > 8 * n
+        _refused(f.ns_embedding_backward(P, L(0), dtype, P, 0, P, 2, L(n), L(1), cols, C.c_float(1), P, z, None), "workspace")
