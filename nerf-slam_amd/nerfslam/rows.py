@@ -83,7 +83,7 @@ def _ids(op, ids):
     if ids.dtype not in (torch.int32, torch.int64):
         _fail(op, f"ids are {ids.dtype}: int32 or int64 are supported")
     if not ids.is_contiguous():
-        raise RuntimeError("ids must be contiguous")
+        _fail(op, "ids must be contiguous")
     return int(ids.dtype == torch.int64)
 
 

@@ -46,3 +46,10 @@ def test_the_largest_gradients_grids():
     for n, cols, dtype in (((1 << 25) - 512, 65536, 2), (1 << 25, 65280, 2), (1 << 25, 65536, 1), (1 << 25, 65536, 3)):
         assert size(L(n), L(1), cols, dtype) > 8 * n
         _refused(f.ns_embedding_backward(P, L(0), dtype, P, 0, P, 2, L(n), L(1), cols, C.c_float(1), P, z, None), "workspace")
+
+
+def test_every_refusal_is_the_frameworks_error():
+    x, ids = torch.zeros(6, 4), torch.zeros(2, 3, dtype=torch.int64).t()
+    for call in (lambda: rows.embedding(x, ids), lambda: rows.embedding_backward(torch.zeros(3, 2, 4), ids, 5)):
+        with pytest.raises(NerfSlamHipError, match="ids must be contiguous"):
+            call()
