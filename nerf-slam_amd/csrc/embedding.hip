@@ -2,27 +2,31 @@
 //
 //   forward    out[t] = round(scale * table[id_t])
 //   gradient   grad[r] = round(scale * sum over t with id_t = r of dout[t])       (rows that no token names: 0)
-// An id outside [0, rows) is a padded place: its output row is zero and its upstream gradient is not read.
+// An id outside [0, rows) is a padded place: its output row is zero and its upstream gradient is not used (it may be read: the sums load
+// every place of the sorted list, and what belongs to no row goes nowhere).
 //
 // The gradient is a sum over the tokens SORTED by id, without floating-point atomics: the order of every sum is fixed by the ids
 // alone, so the same inputs give the same bits.  All sorts are stable.  Three forms, by sizes (times of one call on the device):
 //   short list   n <= SMALL_MAX: one launch; a workgroup owns neighbouring rows of the table and picks their tokens out of the whole list
 //                (embed_small_kernel; 3001 tokens of 771 f32, 1013 rows: 11 us)
 //   few rows     up to FEW_ROWS rows of up to 16 lanes: two launches; a workgroup sorts and sums a tile of tokens, then the tiles' sums are
-//                added per row (embed_tile_kernel, embed_rows_kernel; 262144 tokens of 32 f16, 512 rows: 14 us, 28 in the next form)
+//                added per row (embed_tile_kernel, embed_rows_kernel; 262144 tokens of 32 f16, 512 rows: 14 us, 26 in the next form)
 //   general      sort, sums over equal shares of the sorted list -- so that a row that a tenth of the tokens name costs no more than any
-//                other --, join (16384 tokens of 1024 bf16, 50000 rows: 40 us = 3.4 TB/s of its 135 MB)
+//                other --, join (50000 rows of bf16: 16384 tokens of 1024 40 us = 3.4 TB/s of its 135 MB, 65536 tokens of 1024
+//                80 us = 2.9, of 2048 126 us = 3.7)
 //     sort   n <= RANK_MAX: one launch, a token's place counted directly (embed_rank_kernel); longer: radix passes of up to 10 bits, one
 //            launch each up to ONE_MAX tokens (embed_pass_kernel), beyond as histogram, prefix, scatter
 //     sums   a group of lanes walks consecutive places and sums runs of equal ids in f32 registers (emb_sum_share); a run inside the
 //            workgroup's share is final, one that crosses its ends leaves one f32 partial row per share (embed_sum_kernel)
 //     join   the share in which a crossing run begins adds its partial rows in order (embed_join_kernel)
 // The general form moves little more than dout and the gradient; beside them it is bound by the latency of its launches, each a chain of
-// dependent loads (sort 24 us with the gradient's zeros written beside it, sums 11, join 4 of the 40).
+// dependent loads (16384 tokens of 1024: sort 24 us with the gradient's zeros written beside it, sums 11, join 4 of the 40; 65536 tokens:
+// sort 35 us in six launches, sums 31, join 4).
 //
 // Columns: a lane holds V of them, 16 bytes, or one where a row is shorter than 16 bytes.  The last piece of a row ends with the row, so
 // where D is no multiple of V it overlaps the one before: both lanes form the same sums in the same order and store the same bits.
-// Outputs are stored past the caches (16384 tokens / 50000 rows of 1024 bf16: 72 -> 58 us; lookup of 65536 tokens of 2048: 153 -> 87).
+// Outputs are stored past the caches (lookup of 65536 tokens of 2048 bf16: 87 -> 59 us; the gradient hardly minds, 65536 tokens of 512 bf16 with
+// 32000 f32 rows: 58 -> 56).
 #include "rows.h"
 
 // ---- short list ----
@@ -33,20 +37,25 @@
                              // allowed (beyond, the general form)
 #define SMALL_LANES 4        // log2 of the most lanes per row: a row that takes all of 4096 tokens of 1024 bf16 costs 21 us, with 64 lanes 55
 // ---- few rows ----
-#define FEW_ROWS (MAX_BINS - 1)   // 1000 rows, 262144 tokens of 64 f16 in random order: 28 us against 35 in the general form
-#define FEW_LANES 4          // log2 of the most lanes per row.  At 4 (128 f16, 262144 tokens): 24 against 33 us in runs of 64 equal ids, 42
-                             // against 37 in random order; 32768 tokens: 13 / 21 against 32 / 25.  At 5 random order loses everywhere
-#define FEW_TILES 1024       // 2^20 tokens: 46 against 71 us; bounds the workspace
-#define FEW_WAVES 8          // per tile; 4 or 16: 14.4 or 14.6 us instead of 13.6
-// ---- general ----
-#define RANK_MAX 8192        // 6000 / 8192 tokens: 19 / 22 us against 22 / 23 with radix passes; 16384: 61 against 51
-#define ONE_MAX 16384        // 16384 tokens, two passes: 51 us against 56 as three launches a pass; 32768: 44 against 41
+#define FEW_ROWS (MAX_BINS - 1)   // 1000 rows, 262144 tokens of 64 f16 in random order: 29 us against 33 in the general form
+#define FEW_LANES 4          // log2 of the most lanes per row: what is best depends on the ids' order, which the host does not know.  At 4 (128
+                             // f16 columns) 262144 tokens take 24 against 33 us in runs of 64 equal ids, 42 against 38 in random order; 32768
+                             // tokens 13 against 22 and 21.5 against 23.  At 5 (256 columns) 131072 tokens would take 24 against 33 in runs,
+                             // 52 against 35 in random order
+#define FEW_TILES 1024       // 2^20 tokens of 32 f16: 45 against 71 us; bounds the workspace
+#define FEW_WAVES 8          // per tile; 4 or 16: 14.3 or 14.6 us instead of 13.7 at 262144 tokens of 32
+// ---- general (50000 rows of bf16 unless stated) ----
+#define RANK_MAX 8192        // 256 columns: 6000 / 8192 tokens 17 / 20 us against 21 / 22.5 with radix passes, 16384 tokens 41 against 30.  8192
+                             // tokens of 1024 columns: 37 against 33, as two passes write the gradient's 102 MB of zeros in two launches
+#define ONE_MAX 16384        // 16384 tokens, two passes: 30 us against 37 as three launches a pass (256 columns), 40 against 47 (1024); 32768
+                             // tokens of 256: 43 against 41, 20000 of 1024: 44.5 against 49.5
 #define TILE 1024            // tokens per workgroup of a radix pass and of the few rows' form
 #define MAX_BITS 10          // of a radix pass' digit
 #define MAX_BINS (1 << MAX_BITS)
-#define SUM_U 8              // rows that a lane has on their way; 16: 78 instead of 61 us at 65536 tokens of 512 (fewer waves fit), 4: equal
+#define SUM_U 8              // rows that a lane has on their way; 16: 86 instead of 56 us at 65536 tokens of 512, 32000 rows (fewer waves fit); 4: 56
 #define GROUP 8              // places of the sorted list per group of lanes, doubled (up to 128) while more than GROUP_WAVES waves are
-#define GROUP_WAVES 2048     // at work.  4096 / 8192 waves: 55 / 54 instead of 49 us at 16384 tokens of 1024
+#define GROUP_WAVES 2048     // at work.  1024 / 4096 / 8192 waves: 41 / 41 / 41 instead of 39.5 us at 16384 tokens of 1024, 53 / 50 / 53 instead of
+                             // 49 at 100000 of 256, 56 / 60.5 / 67 instead of 56 at 65536 of 512, 32000 rows
 
 template <typename I>
 __device__ __forceinline__ unsigned emb_key(I id, unsigned rows) {
@@ -86,8 +95,12 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ ta
 // Rows without tokens: every launch of the sort, a few workgroups bound by latency, also writes a part of the whole gradient with zeros
 // (workgroups from `sort` on); the sums that follow write the rows that have tokens again.
 // ---------------------------------------------------------------------------------------------
-#define FILL_BYTES (1 << 14)     // per workgroup, up to FILL_BLOCKS of them: more stores in flight hold up the sort's loads
-#define FILL_BLOCKS 128          // (16384 tokens of 1024 bf16, 50000 rows: 40 us; 240: 41, 512: 44; with the zeros written by the sums: 46)
+// FILL_BLOCKS workgroups at most: more stores in flight hold up the sort's loads, fewer do not get the zeros written meanwhile.  64 / 256 / 512
+// of them: 50000 rows of 1024 bf16 (102 MB), 16384 tokens 39 / 42 / 41 instead of 39.5 us, 65536 tokens 84 / 80.5 / 81 instead of 80; of 2048
+// (205 MB) 143 / 128 / 129 instead of 126; 300000 rows of 1024 f32 (1.2 GB), 16384 tokens 267 / 252 / 266 instead of 250, 65536 tokens 376 / 278 /
+// 293 instead of 262.  (In the form before, the sums wrote the zeros: 46 us for the first.)
+#define FILL_BYTES (1 << 14)     // per workgroup
+#define FILL_BLOCKS 128
 struct EmbFill {
   char* at;
   long bytes;      // of whole elements

@@ -9,7 +9,8 @@
 // registers over all the rows that a workgroup takes, so they cost one partial row pair per workgroup and a second, small launch that
 // adds those in a fixed order: no atomics, the same bits on every run.  All sums are f32; every output is rounded once.
 // Measured (copies of this size run at 5.0 .. 5.4 TB/s): forward 16384 x 4096 bf16 46 us = 5.8 TB/s (parts of it stay in the caches), 230400 x
-// 128 f16 20 us = 6.0; backward 81 us = 5.0 TB/s and 36 us = 4.9.
+// 128 f16 20 us = 6.0; backward 81 us = 5.0 TB/s and 36 us = 4.9.  f32: forward 8192 x 4096 44 us = 6.1 TB/s, 30000 x 771 35 us = 5.3, 2048 x 16384
+// 49 us = 5.5; backward 77 us = 5.3 TB/s, 53 us = 5.3, 93 us = 4.3 (sixteen waves of four pieces a lane: no row fetched ahead).
 #include "rows.h"
 
 #define LN_MAX_COLS 16384
@@ -63,7 +64,10 @@ constexpr int ln_block() { return LPR > 64 ? LPR : 256; }
 
 // ---------------------------------------------------------------------------------------------
 // forward.  Two sums over the row, in turn: the mean, then sum d and sum d^2 of the deviations d = x - mean.  The first of these is what
-// rounding left of the mean; taking it out again keeps the deviations exact where |mean| is far above the row's spread.
+// rounding left of the mean; taking it out again keeps the deviations exact where |mean| is far above the row's spread.  The stored mean is the
+// corrected one: closer than the first where |mean| is above the spread (f32 rows of 128: 5e-8 of the mean at most against 1.2e-7).  Where it is
+// below and the first sum was exact (f16 rows of 128), the correction is nothing but the deviations' rounding, and the stored mean is off by 2^-24 of
+// the spread where the first alone would be right -- what the output's own deviations carry anyway.
 // ---------------------------------------------------------------------------------------------
 template <typename T, typename W, int V, int LPR, int NV>
 __global__ __launch_bounds__(ln_block<LPR>()) void layer_norm_fwd_kernel(const T* __restrict__ x, long xstride, const W* __restrict__ w,
@@ -344,7 +348,7 @@ static void ln_shape(int D, F g) {
   else if (pieces <= 256) f(LnInt<128>(), LnInt<2>());
   else if (pieces <= 512) f(LnInt<256>(), LnInt<2>());
   else if (pieces <= 1024) f(LnInt<512>(), LnInt<2>());
-    else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
+  else if (pieces <= 2048) f(LnInt<1024>(), LnInt<2>());
   else if constexpr (V == 4) f(LnInt<1024>(), LnInt<4>());
 }
 
