@@ -151,9 +151,8 @@ def _weights(op, x, weight, bias):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, stats=False):
     """(x - mean) * rstd * weight + bias over the last axis (at most 16384 wide), rstd = 1 / sqrt(var + eps) with the biased variance;
-    weight / bias [D] in x's dtype or float32, each may be None; eps positive.  Sums and squares are f32: rows of values beyond about 1e18 overflow
-    them.  stats=True: (y, mean, rstd), the latter two float32 of x.shape[:-1] --
-    what `layer_norm_backward` takes."""
+    weight / bias [D] in x's dtype or float32, each may be None; eps positive.  Sums of squares are f32: rows of values beyond about 1e17 overflow
+    them.  stats=True: (y, mean, rstd), the latter two float32 of x.shape[:-1] -- what `layer_norm_backward` takes."""
     op = "layer_norm"
     n, stride = _rows_of(op, "x", x)
     wdtype = _weights(op, x, weight, bias)
