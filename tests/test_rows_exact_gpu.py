@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from nerfslam import rows
-from nerfslam._lib import check, lib, ptr, stream_ptr
+from nerfslam._lib import check, graph_capture, lib, ptr, stream_ptr
 from test_rows_gpu import BF16, F16, F32, U, check_norm, check_norm_backward, gen, half, make_ids, norm64, randn, tiny, within
 
 pytestmark = pytest.mark.gpu
@@ -210,3 +210,30 @@ def test_a_bias_alone_writes_nothing_else(dev):
             want = rows.layer_norm_backward(dout, x, mean, rstd, weight, w)
             assert torch.equal(dx, want[0]) and torch.equal(sums[65:65 + d], want[2] if weight is None else want[1])
             assert bool((sums[:65] == 7).all()) and bool((sums[65 + d:] == 7).all()) and bool((ws[need:] == 0x5a).all())
+
+
+@pytest.mark.parametrize("n,d", [(40, 96), (3000, 96)])
+def test_a_bias_alone_captured_and_replayed(dev, n, d):
+    """in one launch and with partial rows: replayed on new inputs, eager calls and synchronizations between the replays"""
+    g = gen(dev, n)
+    b = 0.1 * randn(g, d)
+    sets = [(randn(g, n, d, dtype=BF16), randn(g, n, d, dtype=BF16)) for _ in range(3)]
+
+    def both(x, dout):
+        y, mean, rstd = rows.layer_norm(x, None, b, stats=True)
+        dx, _, db = rows.layer_norm_backward(dout, x, mean, rstd, None, b)
+        return y, dx, db
+
+    live = [t.clone() for t in sets[0]]
+    both(*live)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with graph_capture(graph):
+        out = both(*live)
+    for turn in range(4):
+        for t, new in zip(live, sets[turn % 3]):
+            t.copy_(new)
+        graph.replay()
+        want = both(*sets[turn % 3])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), turn
